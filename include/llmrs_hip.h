@@ -98,6 +98,14 @@ int llmrs_tensor_upload_q8_0(const int8_t* qs, const float* scales, size_t n,
 int llmrs_tensor_zeros(const size_t* dims, int ndim, llmrs_tensor** out);
 /* Tensor::data() / to_device(Cpu) for f32 tensors: copies `count` floats. */
 int llmrs_tensor_download(const llmrs_tensor* t, float* out, size_t count);
+/* Device memory of another library in this process (no reference counterpart).
+ * copy_device: a new f32 tensor from contiguous f32 values in device memory.
+ * Waits for all work queued on that device, whatever its stream, and for the
+ * copy, so `src` may be reused on return.  address: where an f32 tensor's values
+ * are, valid until llmrs_tensor_free; work queued by this library may still be
+ * writing there until llmrs_sync. */
+int llmrs_tensor_copy_device(const void* src, const size_t* dims, int ndim, llmrs_tensor** out);
+int llmrs_tensor_address(const llmrs_tensor* t, void** address);
 int llmrs_tensor_ndim(const llmrs_tensor* t);
 int llmrs_tensor_dims(const llmrs_tensor* t, size_t* dims);
 int llmrs_tensor_dtype(const llmrs_tensor* t);
@@ -387,6 +395,80 @@ int llmrs_batch_tokens(llmrs_batch* b, int32_t slot, int32_t* out, size_t count)
 int llmrs_batch_logits(llmrs_batch* b, float* out);
 /* Per-launch timing of one eager batched step (as llmrs_model_profile_step). */
 int llmrs_batch_profile_step(llmrs_batch* b, char* names, float* ms, double* work, int cap);
+
+/* ---- paged 8-bit K/V cache (no reference counterpart) ----------------------
+ * One pool of pages that many sequences share, for one layer: each sequence
+ * (a slot) holds the pages mapped to it, in order, and a length.  Keys and
+ * values are 8-bit codes with a power-of-two scale for every block of 32
+ * positions, KV head and K or V: value = code * 2^e, e the smallest exponent in
+ * [-100, 121] for which the largest magnitude of the block's rows is at most
+ * 127 * 2^e.  Rows that join a block may raise e; the codes already there are
+ * rounded to the new step (half to even).  Truncating leaves e as it is; a block
+ * that is begun again starts afresh.  NaN is stored as zero, larger magnitudes
+ * as 127 * 2^121.
+ *
+ * The page table and the lengths are checked and kept on the host: a call with
+ * an unknown slot, a slot named twice, a page in use, or positions without a
+ * page is refused and changes nothing.  Device memory is taken by the first
+ * append.  Calls are queued on the library's stream and do not wait. */
+typedef struct llmrs_paged llmrs_paged;
+typedef struct {
+  int32_t n_kv_heads;  /* 1 to 256 */
+  int32_t head_dim;    /* 64 or 128 */
+  int32_t page_size;   /* positions per page: a power of two, 32 to 4096 */
+  int32_t n_pages;     /* pages of the pool */
+  int32_t max_seqs;    /* slots */
+  int32_t max_seq;     /* positions of a sequence, at most 1048576 */
+  float rope_theta;    /* rotation base; 0 and no tables: no rotation */
+} llmrs_paged_config;
+/* rope_cos, rope_sin: the rotation's tables [max_seq][head_dim/2], or both NULL
+ * for those of rope_theta (as llmrs_rope_inplace computes them).  Dimension
+ * j < head_dim/2 turns with j + head_dim/2. */
+int llmrs_paged_create(const llmrs_paged_config* cfg, const float* rope_cos, const float* rope_sin, llmrs_paged** out);
+int llmrs_paged_free(llmrs_paged* p);
+/* Adds n pages at the end of a slot's.  A page belongs to one slot at a time. */
+int llmrs_paged_map(llmrs_paged* p, int32_t slot, const int32_t* pages, size_t n);
+/* Ends a slot's sequence: length 0, its pages free. */
+int llmrs_paged_release(llmrs_paged* p, int32_t slot);
+int llmrs_paged_length(const llmrs_paged* p, int32_t slot, int32_t* length);
+/* Shortens sequences (drafted tokens that were refused). */
+int llmrs_paged_truncate(llmrs_paged* p, const int32_t* slots, const int32_t* lengths, size_t n);
+/* Appends counts[i] rows to slots[i], for n sequences: k and v are f32
+ * [sum of counts][n_kv_heads * head_dim], the sequences' rows one after the
+ * other.  rotate != 0: k is rotated to its positions (in 64 bits); 0: k is
+ * rotated already. */
+int llmrs_paged_append(llmrs_paged* p, const llmrs_tensor* k, const llmrs_tensor* v, const int32_t* slots,
+                       const int32_t* counts, size_t n, int rotate);
+/* Rows [starts[i], starts[i] + counts[i]) of slots[i] as the cache holds them,
+ * f32 [sum of counts][n_kv_heads * head_dim]. */
+int llmrs_paged_read(llmrs_paged* p, const int32_t* slots, const int32_t* starts, const int32_t* counts, size_t n,
+                     llmrs_tensor** k, llmrs_tensor** v);
+/* Causal attention of the last counts[i] positions of slots[i], already
+ * appended: q f32 [sum of counts][query heads * head_dim], not rotated; *out the
+ * same shape.  Row t of a sequence of length L and count c sits at position p =
+ * L - c + t: softmax over the positions up to p of (rotated q . K) / sqrt(head_dim),
+ * times V.  Query head h reads KV head h / (query heads / KV heads). */
+int llmrs_paged_attention(llmrs_paged* p, const llmrs_tensor* q, const int32_t* slots, const int32_t* counts, size_t n,
+                          llmrs_tensor** out);
+
+/* ---- verification of drafted tokens (no reference counterpart) -------------
+ * For n sequences with counts[i] (0 to 64) drafted tokens each: `target` f32
+ * [sum of (counts[i] + 1)][vocab] holds the target's probabilities before each
+ * draft and after the last, `draft` f32 [sum of counts][vocab] those that each
+ * draft came from (NULL: the drafts are certain, probability 1), `ids` and
+ * `accept` one id and one uniform number in [0, 1] per draft, `draw` one in
+ * [0, 1) per sequence.  Draft x is accepted while accept * draft[x] <
+ * target[x] (exactly).  The first refused one is replaced by a draw from
+ * max(target - draft, 0); after the last accepted one a token is drawn from the
+ * target's last row.  A draw takes the smallest id whose running sum in 64 bits
+ * exceeds draw * total; where nothing is left of the target, from the target as
+ * it is.  NaN counts as zero; a row with nothing in it gives the last id.
+ * Writes per sequence the number of accepted drafts and, in a row of `width` >=
+ * largest count + 1 ids, these, the drawn id and -1 for the rest.  Returns when
+ * they are there. */
+int llmrs_verify_drafts(const llmrs_tensor* target, const llmrs_tensor* draft, const int32_t* ids,
+                        const int32_t* counts, const float* accept, const float* draw, size_t n,
+                        int32_t* accepted, int32_t* tokens, size_t width);
 
 /* ---- test probes (no reference counterpart) ------------------------------
  * One layer's kernels run on inputs given by the host, with every

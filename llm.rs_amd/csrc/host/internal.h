@@ -80,6 +80,7 @@ struct Context {
   std::string noalloc_error;        // why it is null
   uint8_t* host_out = nullptr;      // pinned: what fetch brings back (kFetchBytes + 64)
   std::vector<hipModule_t> modules;
+  std::vector<std::string> module_names;
   std::map<std::string, KernelInfo> kernels;
   Allocator alloc;
 };

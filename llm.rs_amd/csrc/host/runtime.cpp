@@ -45,7 +45,16 @@ hipFunction_t kernel(const std::string& name, dim3 block) {
   Context& c = ctx();
   auto it = c.kernels.find(name);
   if (it == c.kernels.end()) {
-    for (hipModule_t m : c.modules) {
+    // most kernels carry their module's name in front, and the rest are operators:
+    // asking another module first would leave its "not found" as the thread's last
+    // HIP error
+    const std::string tag = name.substr(0, name.find('_'));
+    std::vector<hipModule_t> order;
+    for (const std::string& first : {tag, std::string("ops")})
+      for (size_t i = 0; i < c.modules.size(); ++i)
+        if (c.module_names[i] == first) order.push_back(c.modules[i]);
+    order.insert(order.end(), c.modules.begin(), c.modules.end());
+    for (hipModule_t m : order) {
       KernelInfo k;
       if (hipModuleGetFunction(&k.f, m, name.c_str()) == hipSuccess && k.f) {
         LLMRS_HIP(hipFuncGetAttribute(&k.max_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, k.f));
@@ -471,7 +480,7 @@ int llmrs_init(int device_ordinal, const char* hsaco_dir) {
         c->noalloc_error = e.what();
       }
       std::string dir = hsaco_dir ? std::string(hsaco_dir) : library_dir();
-      for (const char* name : {"gemv", "gemv_w8", "attention", "exact", "ops", "prefill", "sample", "sgemm"}) {
+      for (const char* name : {"gemv", "gemv_w8", "attention", "exact", "ops", "paged", "prefill", "sample", "sgemm", "verify"}) {
         std::string path = dir + "/" + name + ".hsaco";
         LLMRS_REQUIRE(std::filesystem::exists(path), LLMRS_E_MODULE, "missing code object " + path);
         hipModule_t m = nullptr;
@@ -479,6 +488,7 @@ int llmrs_init(int device_ordinal, const char* hsaco_dir) {
         if (e != hipSuccess)
           fail(LLMRS_E_MODULE, "hipModuleLoad(" + path + "): " + hipGetErrorString(e));
         c->modules.push_back(m);
+        c->module_names.push_back(name);
       }
     } catch (...) {
       for (hipModule_t m : c->modules) (void)hipModuleUnload(m);

@@ -3,7 +3,7 @@
 #include <memory>
 
 #include "../kernel_args.h"
-#include "internal.h"
+#include "words.h"
 
 using namespace llmrs;
 
@@ -133,6 +133,51 @@ int llmrs_tensor_download(const llmrs_tensor* t, float* out, size_t count) {
     LLMRS_REQUIRE(count == t->numel(), LLMRS_E_INVALID, "download count != numel");
     LLMRS_REQUIRE(out || !count, LLMRS_E_INVALID, "out is null");
     fetch(out, t->data, count * sizeof(float));
+  });
+}
+
+int llmrs_tensor_copy_device(const void* src, const size_t* dims, int ndim, llmrs_tensor** out) {
+  return guard([&] {
+    LLMRS_REQUIRE(out, LLMRS_E_INVALID, "out is null");
+    const std::vector<size_t> d = dims_of(dims, ndim);
+    size_t count = 1;
+    for (size_t x : d) {
+      LLMRS_REQUIRE(!x || count <= ((size_t)1 << 40) / x, LLMRS_E_INVALID, "copy_device: too large");
+      count *= x;
+    }
+    (void)ctx();
+    OnDevice here;
+    if (count) {
+      hipPointerAttribute_t at;
+      hipDeviceptr_t base = nullptr;
+      size_t size = 0;
+      const bool known = src && hipPointerGetAttributes(&at, src) == hipSuccess && at.type == hipMemoryTypeDevice &&
+                         hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)src) == hipSuccess;
+      if (!known) (void)hipGetLastError();
+      LLMRS_REQUIRE(known && (const char*)src + 4 * count <= (const char*)base + size, LLMRS_E_INVALID,
+                    "copy_device: not " + std::to_string(4 * count) + " bytes of device memory");
+      // whatever stream the data is being written on
+      LLMRS_HIP(hipSetDevice(at.device));
+      const hipError_t e = hipDeviceSynchronize();
+      LLMRS_HIP(hipSetDevice(ctx().device));
+      LLMRS_HIP(e);
+    }
+    std::unique_ptr<llmrs_tensor> t(alloc_f32(d));
+    if (count) {
+      hipError_t e = hipMemcpyAsync(t->data, src, t->bytes, hipMemcpyDefault, ctx().stream);
+      if (e == hipSuccess) e = hipStreamSynchronize(ctx().stream);
+      if (e != hipSuccess) ctx().alloc.release(t->data);
+      LLMRS_HIP(e);
+    }
+    *out = t.release();
+  });
+}
+
+int llmrs_tensor_address(const llmrs_tensor* t, void** address) {
+  return guard([&] {
+    require_f32(t, "address");
+    LLMRS_REQUIRE(address, LLMRS_E_INVALID, "address is null");
+    *address = t->data;
   });
 }
 

@@ -1,0 +1,85 @@
+// verify.cpp - llmrs_verify_drafts: drafted tokens against the target's
+// probabilities (verify.hip).
+#include <cstring>
+
+#include "words.h"
+
+using namespace llmrs;
+
+namespace {
+
+void require_rows(const llmrs_tensor* t, size_t rows, size_t vocab, const char* what) {
+  LLMRS_REQUIRE(t->dtype == LLMRS_F32, LLMRS_E_DTYPE, std::string("verify_drafts: ") + what + " must be an f32 tensor");
+  LLMRS_REQUIRE(t->dims.size() == 2 && t->dims[0] == rows && t->dims[1] == vocab, LLMRS_E_INVALID,
+                std::string("verify_drafts: ") + what + " must be [" + std::to_string(rows) + ", " + std::to_string(vocab) + "]");
+}
+
+}  // namespace
+
+extern "C" int llmrs_verify_drafts(const llmrs_tensor* target, const llmrs_tensor* draft, const int32_t* ids,
+                                   const int32_t* counts, const float* accept, const float* draw, size_t n,
+                                   int32_t* accepted, int32_t* tokens, size_t width) {
+  return guard([&] {
+    if (!n) return;
+    LLMRS_REQUIRE(target && counts && draw && accepted && tokens, LLMRS_E_INVALID, "verify_drafts: null argument");
+    LLMRS_REQUIRE(n <= 65535, LLMRS_E_INVALID, "verify_drafts: at most 65535 sequences");
+    LLMRS_REQUIRE(target->dims.size() == 2 && target->dims[1] > 0 && target->dims[1] <= ((size_t)1 << 30), LLMRS_E_INVALID,
+                  "verify_drafts: target must be [rows, vocabulary]");
+    const size_t vocab = target->dims[1];
+    size_t total = 0, most = 0;
+    std::vector<int> w(3 * n);
+    for (size_t i = 0; i < n; ++i) {
+      LLMRS_REQUIRE(counts[i] >= 0 && counts[i] <= kVerifyMaxDrafts, LLMRS_E_RANGE,
+                    "verify_drafts: sequence " + std::to_string(i) + " has " + std::to_string(counts[i]) + " drafts (0 to " +
+                        std::to_string(kVerifyMaxDrafts) + ")");
+      w[3 * i] = (int)(total + i);
+      w[3 * i + 1] = (int)total;
+      w[3 * i + 2] = counts[i];
+      total += (size_t)counts[i];
+      most = std::max(most, (size_t)counts[i]);
+    }
+    require_rows(target, total + n, vocab, "target");
+    if (draft) require_rows(draft, total, vocab, "draft");
+    LLMRS_REQUIRE(!total || (ids && accept), LLMRS_E_INVALID, "verify_drafts: null argument");
+    LLMRS_REQUIRE(width > most, LLMRS_E_INVALID,
+                  "verify_drafts: rows of " + std::to_string(width) + " tokens cannot hold " + std::to_string(most) +
+                      " drafts and the next token");
+    for (size_t j = 0; j < total; ++j) {
+      LLMRS_REQUIRE(ids[j] >= 0 && (size_t)ids[j] < vocab, LLMRS_E_RANGE,
+                    "verify_drafts: drafted id " + std::to_string(ids[j]) + " outside the vocabulary");
+      LLMRS_REQUIRE(accept[j] >= 0.0f && accept[j] <= 1.0f, LLMRS_E_INVALID, "verify_drafts: accept outside [0, 1]");
+    }
+    for (size_t i = 0; i < n; ++i)
+      LLMRS_REQUIRE(draw[i] >= 0.0f && draw[i] < 1.0f, LLMRS_E_INVALID, "verify_drafts: draw outside [0, 1)");
+    Context& c = ctx();
+    OnDevice here;
+    w.insert(w.end(), ids, ids + total);
+    const size_t at = w.size();
+    w.resize(at + total + n);
+    if (total) std::memcpy(&w[at], accept, 4 * total);
+    std::memcpy(&w[at + total], draw, 4 * n);
+
+    VerifyArgs a;
+    a.target = (const float*)target->data;
+    a.draft = draft ? (const float*)draft->data : nullptr;
+    a.vocab = (int)vocab;
+    a.n = (int)n;
+    a.groups = verify_groups((int)vocab);
+    a.most = (int)most;
+    a.drafts = (int)total;
+    const size_t row = 2 + most;
+    Scratch part(16 * n * (size_t)a.groups), out(4 * n * row);
+    a.part = (double*)part.p;
+    a.out = (int*)out.p;
+    LaunchWords words(w, a.w);
+    a.ext = words.ext();
+    launch("verify_sums", dim3((unsigned)a.groups, (unsigned)n), dim3(256), 0, c.stream, a);
+    launch("verify_pick", dim3((unsigned)n), dim3(256), 0, c.stream, a);
+    std::vector<int> got(n * row);
+    fetch(got.data(), out.p, 4 * got.size());
+    for (size_t i = 0; i < n; ++i) {
+      accepted[i] = got[i * row];
+      for (size_t j = 0; j < width; ++j) tokens[i * width + j] = j <= most ? got[i * row + 1 + j] : -1;
+    }
+  });
+}

@@ -452,4 +452,92 @@ constexpr size_t attn_lds_bytes(int hd, bool kv16, int streams = 1) {
   return 4 * 8 * (size_t)hd + (size_t)streams * stream + 4 * 2 * (size_t)hd + 16;
 }
 
+// ---- paged 8-bit K/V cache (paged.hip) -------------------------------------
+// Positions that share a scale: a value is code * 2^e, one exponent per block,
+// KV head and K or V.  Rows of [pool block][KV head][K | V][codes].
+constexpr int kPagedBlock = 32;
+constexpr int kPagedExpMin = -100, kPagedExpMax = 121;  // 127 * 2^121 is finite in f32
+constexpr size_t paged_block_bytes(int nkv, int hd) { return (size_t)nkv * 2 * kPagedBlock * hd; }
+// Where a code stands in its block, so that a matrix-core operand is 16
+// consecutive bytes of a lane.  K: operand rows b = 0..3 of a 64-position tile
+// hold positions 16 (c / 4) + 4 b + c % 4 (c = 0..15, eight of them in each of the
+// tile's two blocks), dims in steps of 64 and lane groups of 16; with 64 dims a
+// group's bytes are dims 8 r .. 8 r + 7 and their rotation partners 32 further on.
+constexpr int paged_k_offset(int p, int d, int hd) {
+  const int s = hd == 128 ? d >> 6 : 0, r = hd == 128 ? (d >> 4) & 3 : (d & 31) >> 3;
+  const int e = hd == 128 ? d & 15 : (d & 7) + (d >> 5) * 8;
+  return (((((p >> 2) & 3) * (hd / 64) + s) * 4 + r) * 8 + (p >> 4) * 4 + (p & 3)) * 16 + e;
+}
+// V: operand rows are 16 dims, a lane's bytes 16 consecutive positions.  Its codes
+// are stored plus 128.
+constexpr int paged_v_offset(int p, int d) { return (((d >> 4) * 2 + (p >> 4)) * 16 + (d & 15)) * 16 + (p & 15); }
+
+// What a launch knows of its sequences: kPagedWords 32-bit words in its own
+// arguments, more in device memory (`ext`).  First the n sequences' first work
+// items, then per sequence its slot, first row, rows and positions.
+constexpr int kPagedWords = 480;
+constexpr int kPagedPerSeq = 5;
+struct PagedSeqs {
+  const int* ext;
+  int n, items;
+  int w[kPagedWords];
+};
+
+// Words into device memory (paged.hip: paged_words).
+struct WordsArgs {
+  int* dst;
+  int n;
+  int w[kPagedWords];
+};
+
+struct PagedPool {
+  uint8_t* codes;        // [pool block][KV head][2][kPagedBlock * hd]
+  int8_t* exps;          // [pool block][KV head][2]
+  const int* table;      // [slot][stride] pages
+  int stride, shift;     // shift: log2 of the blocks per page
+  int nkv;
+};
+
+// Append (rows in) and read (rows out): a work item is one block of one
+// sequence, over (item, KV head, K or V).
+struct PagedRowsArgs {
+  PagedPool pool;
+  float* rows[2];        // K, V rows [rows][nkv * hd]
+  const float* rope_cos; // [positions][hd / 2]; null: as they are
+  const float* rope_sin;
+  PagedSeqs seqs;        // positions: before the new rows (append), of the first row (read)
+};
+
+// Attention of new rows.  A work item is a tile of (row, query head of the group)
+// columns and a split of `chunk` positions; items of one tile follow each other.
+struct PagedAttnArgs {
+  PagedPool pool;
+  const float* q;        // [rows][nq * hd]
+  float* out;            // [rows][nq * hd]
+  float* part_o;         // [item][KV head][columns][hd] (splits)
+  float* part_ml;        // [item][KV head][columns][2]
+  const float* rope_cos; // null: q as it is
+  const float* rope_sin;
+  int nq, chunk;
+  float scale;           // 1 / sqrt(hd)
+  PagedSeqs seqs;        // positions: with the new rows
+};
+
+// ---- verification of drafted tokens (verify.hip) -----------------------------
+constexpr int kVerifySlice = 2048;  // ids per workgroup
+constexpr int kVerifyMaxDrafts = 64;
+constexpr int verify_groups(int vocab) { return (vocab + kVerifySlice - 1) / kVerifySlice; }
+struct VerifyArgs {
+  const float* target;   // [rows][vocab]
+  const float* draft;    // [drafted rows][vocab] (null: probability 1 at the drafted id)
+  double* part;          // [sequence][group][2] sums of a slice: what is left of the target, the target
+  int* out;              // [sequence][2 + most]: accepted, then its tokens (-1 past the last)
+  int vocab, n, groups, most;
+  // words (as PagedSeqs): per sequence its first target row, first drafted row and
+  // drafts; then the drafted ids, their uniform numbers (f32 bits), the draws
+  const int* ext;
+  int drafts;            // of all sequences
+  int w[kPagedWords];
+};
+
 }  // namespace llmrs

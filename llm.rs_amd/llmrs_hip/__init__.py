@@ -65,6 +65,8 @@ _SIGS = {
     "llmrs_tensor_upload_q8_0": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.POINTER(C.c_void_p)]),
     "llmrs_tensor_zeros": (C.c_int, [C.POINTER(C.c_size_t), C.c_int, C.POINTER(C.c_void_p)]),
     "llmrs_tensor_download": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t]),
+    "llmrs_tensor_copy_device": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t), C.c_int, C.POINTER(C.c_void_p)]),
+    "llmrs_tensor_address": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "llmrs_tensor_ndim": (C.c_int, [C.c_void_p]),
     "llmrs_tensor_dims": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t)]),
     "llmrs_tensor_dtype": (C.c_int, [C.c_void_p]),
@@ -127,6 +129,19 @@ _SIGS = {
                                           C.c_void_p]),
     "llmrs_model_probe_prefill_layer": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_void_p,
                                                    C.c_void_p]),
+    "llmrs_paged_create": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
+    "llmrs_paged_free": (C.c_int, [C.c_void_p]),
+    "llmrs_paged_map": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_size_t]),
+    "llmrs_paged_release": (C.c_int, [C.c_void_p, C.c_int32]),
+    "llmrs_paged_length": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(C.c_int32)]),
+    "llmrs_paged_truncate": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
+    "llmrs_paged_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int]),
+    "llmrs_paged_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p),
+                                   C.POINTER(C.c_void_p)]),
+    "llmrs_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                        C.POINTER(C.c_void_p)]),
+    "llmrs_verify_drafts": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                      C.c_void_p, C.c_void_p, C.c_size_t]),
     "llmrs_synth_q4": (C.c_int, [C.c_uint64, C.c_uint64, C.c_size_t, C.c_size_t, C.c_float, C.c_float, C.c_void_p, C.c_void_p, C.c_int]),
     "llmrs_synth_q8": (C.c_int, [C.c_uint64, C.c_uint64, C.c_size_t, C.c_size_t, C.c_float, C.c_float, C.c_void_p, C.c_void_p, C.c_int]),
     "llmrs_synth_normal": (C.c_int, [C.c_uint64, C.c_uint64, C.c_size_t, C.c_float, C.c_float, C.c_void_p, C.c_int]),
@@ -260,6 +275,36 @@ class Tensor:
         out = C.c_void_p()
         _check(lib().llmrs_tensor_upload_f32(_ptr(a), dims, max(a.ndim, 1), C.byref(out)))
         return Tensor(out.value)
+
+    @staticmethod
+    def from_device(x) -> "Tensor":
+        """A copy of another library's contiguous f32 array on the GPU
+        (anything with ``__cuda_array_interface__``, e.g. a torch tensor):
+        llmrs_tensor_copy_device."""
+        info = getattr(x, "__cuda_array_interface__", None)
+        if info is None:
+            raise LlmrsError(E_INVALID, "from_device: not an array in device memory")
+        if info["typestr"] != "<f4":
+            raise LlmrsError(E_DTYPE, f"from_device: f32 values, not {info['typestr']}")
+        shape = tuple(info["shape"]) or (1,)
+        dense = [4] * len(shape)
+        for i in range(len(shape) - 2, -1, -1):
+            dense[i] = dense[i + 1] * shape[i + 1]
+        if info.get("strides") and 0 not in shape and any(n > 1 and a != b for n, a, b in zip(shape, info["strides"], dense)):
+            raise LlmrsError(E_INVALID, "from_device: the array is not contiguous")
+        out = C.c_void_p()
+        _check(lib().llmrs_tensor_copy_device(info["data"][0], (C.c_size_t * len(shape))(*shape), len(shape), C.byref(out)))
+        return Tensor(out.value)
+
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        """An f32 tensor's values in place, for another library in this
+        process: while this object lives, and not before ``sync()`` where
+        work on them is still queued."""
+        at = C.c_void_p()
+        _check(lib().llmrs_tensor_address(self._h, C.byref(at)))
+        shape = self.shape
+        return {"shape": shape, "typestr": "<f4", "data": (0 if 0 in shape else at.value, False), "version": 3}
 
     @staticmethod
     def from_q4(qs: np.ndarray, scales: np.ndarray, n: int, k: int) -> "Tensor":
@@ -642,7 +687,6 @@ class HipModel:
                 "exact": bool(out[3])}
 
 
-# -- seeded synthetic inputs (llmrs_synth_*) ------------------------------
 class HipBatch:
     """B sequences of one model decoding together (llmrs_batch_*)."""
 
@@ -691,6 +735,110 @@ class HipBatch:
                 for i in range(n)]
 
 
+class PagedConfig(C.Structure):
+    """llmrs_paged_config."""
+    _fields_ = [("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+                ("max_seqs", C.c_int32), ("max_seq", C.c_int32), ("rope_theta", C.c_float)]
+
+
+def _i32(a) -> np.ndarray:
+    return np.ascontiguousarray(a, dtype=np.int32).reshape(-1)
+
+
+def _pair(a, b, what: str):
+    a, b = _i32(a), _i32(b)
+    if a.size != b.size:
+        raise LlmrsError(E_INVALID, f"{what}: {a.size} slots, {b.size} numbers")
+    return a, b
+
+
+class HipPagedCache:
+    """One layer's paged 8-bit K/V cache of many sequences (llmrs_paged_*)."""
+
+    def __init__(self, n_kv_heads: int, head_dim: int, page_size: int, n_pages: int, max_seqs: int, max_seq: int,
+                 rope=500000.0):
+        """rope: the rotation's base, its tables (cos, sin) [max_seq][head_dim/2],
+        or None for no rotation."""
+        theta, cos, sin = 0.0, None, None
+        if isinstance(rope, (tuple, list)):
+            cos, sin = (np.ascontiguousarray(t, dtype=np.float32) for t in rope)
+            if cos.shape != (max_seq, head_dim // 2) or sin.shape != cos.shape:
+                raise LlmrsError(E_INVALID, "rope tables must be [max_seq][head_dim/2]")
+        elif rope is not None:
+            theta = float(rope)
+        self.cfg = PagedConfig(n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_seq, theta)
+        h = C.c_void_p()
+        _check(lib().llmrs_paged_create(C.byref(self.cfg), _ptr(cos), _ptr(sin), C.byref(h)))
+        self._h = h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            _check(lib().llmrs_paged_free(self._h))
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def map(self, slot: int, pages) -> None:
+        """Adds pages at the end of a slot's."""
+        pages = _i32(pages)
+        _check(lib().llmrs_paged_map(self._h, int(slot), _ptr(pages), pages.size))
+
+    def release(self, slot: int) -> None:
+        """Ends a slot's sequence and frees its pages."""
+        _check(lib().llmrs_paged_release(self._h, int(slot)))
+
+    def length(self, slot: int) -> int:
+        n = C.c_int32()
+        _check(lib().llmrs_paged_length(self._h, int(slot), C.byref(n)))
+        return int(n.value)
+
+    def truncate(self, slots, lengths) -> None:
+        """Shortens sequences to the given lengths."""
+        slots, lengths = _pair(slots, lengths, "truncate")
+        _check(lib().llmrs_paged_truncate(self._h, _ptr(slots), _ptr(lengths), slots.size))
+
+    def append(self, k: Tensor, v: Tensor, slots, counts, rotate: bool = True) -> None:
+        """Appends counts[i] rows of k and v to slots[i], k rotated to its
+        positions on the way (rotate=False: it is already)."""
+        slots, counts = _pair(slots, counts, "append")
+        _check(lib().llmrs_paged_append(self._h, k.handle, v.handle, _ptr(slots), _ptr(counts), slots.size,
+                                        1 if rotate else 0))
+
+    def read(self, slots, starts, counts) -> tuple[Tensor, Tensor]:
+        """Rows [starts[i], starts[i] + counts[i]) of slots[i] as f32: (K, V)."""
+        slots, counts = _pair(slots, counts, "read")
+        slots, starts = _pair(slots, starts, "read")
+        k, v = C.c_void_p(), C.c_void_p()
+        _check(lib().llmrs_paged_read(self._h, _ptr(slots), _ptr(starts), _ptr(counts), slots.size, C.byref(k), C.byref(v)))
+        return Tensor(k.value), Tensor(v.value)
+
+    def attention(self, q: Tensor, slots, counts) -> Tensor:
+        """Causal attention of the last counts[i] positions of slots[i] (already
+        appended); q is rotated on the way."""
+        slots, counts = _pair(slots, counts, "attention")
+        return _out_tensor(lib().llmrs_paged_attention, self._h, q.handle, _ptr(slots), _ptr(counts), slots.size)
+
+
+def verify_drafts(target: Tensor, ids, counts, accept, draw, draft: Tensor | None = None) -> tuple[np.ndarray, np.ndarray]:
+    """Drafted tokens against the target's probabilities, from given uniform
+    numbers (llmrs_verify_drafts): accepted drafts per sequence, and their ids
+    followed by the next token's, -1 past it."""
+    ids, counts = _i32(ids), _i32(counts)
+    accept, draw = (np.ascontiguousarray(a, dtype=np.float32).reshape(-1) for a in (accept, draw))
+    if counts.size and counts.min() < 0 or ids.size != counts.sum() or accept.size != ids.size or draw.size != counts.size:
+        raise LlmrsError(E_INVALID, "verify_drafts: one id and one number per draft, one draw per sequence")
+    width = int(counts.max()) + 1 if counts.size else 1
+    accepted, tokens = np.empty(counts.size, np.int32), np.empty((counts.size, width), np.int32)
+    _check(lib().llmrs_verify_drafts(target.handle, draft.handle if draft is not None else None, _ptr(ids), _ptr(counts),
+                                     _ptr(accept), _ptr(draw), counts.size, _ptr(accepted), _ptr(tokens), width))
+    return accepted, tokens
+
+
+# -- seeded synthetic inputs (llmrs_synth_*) ------------------------------
 def synth_q4(seed: int, tid: int, n: int, k: int, lo: float, hi: float, threads: int = 0):
     qs = np.empty(n * k // 2, np.uint8)
     sc = np.empty(n * k // 32, np.float32)

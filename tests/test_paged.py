@@ -1,0 +1,133 @@
+"""The paged cache and the verification of drafts without a GPU: the layout of a
+block, and every call that is refused before a device is touched."""
+from __future__ import annotations
+
+import ctypes as C
+import shutil
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+import llmrs_hip as lh
+
+HERE = Path(__file__).resolve().parent
+CSRC = HERE.parent / "llm.rs_amd" / "csrc"
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_block_layout(tmp_path):
+    exe = tmp_path / "paged_layout"
+    subprocess.run(["g++", "-O1", "-std=c++17", f"-I{CSRC}", "-o", str(exe), str(HERE / "native" / "paged_layout.cpp")], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "mismatches 0\n"
+
+
+def cache(**kw):
+    args = dict(n_kv_heads=2, head_dim=64, page_size=32, n_pages=6, max_seqs=3, max_seq=100, rope=None) | kw
+    return lh.HipPagedCache(**args)
+
+
+def refused(code, fn, *args, **kw):
+    with pytest.raises(lh.LlmrsError) as e:
+        fn(*args, **kw)
+    assert e.value.code == code, e.value
+    return str(e.value)
+
+
+@pytest.mark.parametrize("kw", [
+    {"head_dim": 96}, {"head_dim": 0}, {"n_kv_heads": 0}, {"n_kv_heads": 257}, {"page_size": 16}, {"page_size": 48},
+    {"page_size": 8192}, {"page_size": -32}, {"n_pages": 0}, {"n_pages": -1}, {"page_size": 4096, "n_pages": 1 << 30},
+    {"max_seqs": 0}, {"max_seqs": 65537}, {"max_seq": 0}, {"max_seq": (1 << 20) + 1},
+    {"max_seqs": 65536, "max_seq": 1 << 20}, {"rope": -1.0}, {"rope": float("nan")}, {"rope": float("inf")},
+])
+def test_bad_configuration(kw):
+    refused(lh.E_INVALID, cache, **kw)
+
+
+def test_bad_tables():
+    c, s = np.zeros((100, 32), np.float32), np.zeros((100, 31), np.float32)
+    refused(lh.E_INVALID, cache, rope=(c, s))
+    refused(lh.E_INVALID, cache, rope=(c[:50], c[:50]))
+    cfg, h = lh.PagedConfig(2, 64, 32, 6, 3, 100, 0.0), C.c_void_p()
+    assert lh.lib().llmrs_paged_create(C.byref(cfg), c.ctypes.data_as(C.c_void_p), None, C.byref(h)) == lh.E_INVALID
+    assert lh.lib().llmrs_paged_create(None, None, None, C.byref(h)) == lh.E_INVALID
+    assert not h.value
+
+
+def test_mapping_pages():
+    c = cache()
+    c.map(0, [4, 2])
+    assert "in use" in refused(lh.E_INVALID, c.map, 1, [2])
+    refused(lh.E_INVALID, c.map, 0, [4])
+    refused(lh.E_INVALID, c.map, 1, [3, 3])       # twice in one call
+    c.map(1, [3])                                 # which took nothing
+    refused(lh.E_RANGE, c.map, 1, [0, 6])
+    refused(lh.E_RANGE, c.map, 1, [0, -1])
+    refused(lh.E_RANGE, c.map, 0, [0, 1, 5])      # 100 positions are four pages
+    refused(lh.E_RANGE, c.map, 3, [0])
+    refused(lh.E_RANGE, c.map, -1, [0])
+    c.map(0, [0, 1])
+    c.map(0, [])
+    c.release(0)
+    c.map(2, [4, 2, 0, 1])
+    assert c.length(2) == 0
+    refused(lh.E_RANGE, c.length, 3)
+    refused(lh.E_RANGE, c.release, 7)
+
+
+def test_lengths_only_shrink():
+    c = cache()
+    refused(lh.E_RANGE, c.truncate, [0], [1])
+    refused(lh.E_RANGE, c.truncate, [0], [-1])
+    refused(lh.E_RANGE, c.truncate, [9], [0])
+    refused(lh.E_INVALID, c.truncate, [0, 0], [0, 0])
+    refused(lh.E_INVALID, c.truncate, [0, 1], [0])
+    c.truncate([0, 2], [0, 0])
+    c.truncate([], [])
+
+
+class NoTensor:
+    handle = None
+
+
+def test_append_read_attention_refusals():
+    """Slots, counts and positions are looked at before any tensor."""
+    c, no = cache(), NoTensor()
+    c.map(0, [0, 1, 2, 3])
+    c.map(1, [5])
+    for call in (c.append, lambda k, v, s, n: c.read(s, n, n), lambda k, v, s, n: c.attention(k, s, n)):
+        refused(lh.E_RANGE, call, no, no, [3], [1])
+        refused(lh.E_RANGE, call, no, no, [-1], [1])
+        refused(lh.E_INVALID, call, no, no, [0, 0], [1, 1])
+        refused(lh.E_RANGE, call, no, no, [0], [-1])
+        refused(lh.E_RANGE, call, no, no, [0], [101])
+        refused(lh.E_INVALID, call, no, no, [0, 1], [1])
+    assert "no page" in refused(lh.E_RANGE, c.append, no, no, [0, 1], [100, 33])
+    assert "no page" in refused(lh.E_RANGE, c.append, no, no, [2], [1])
+    refused(lh.E_INVALID, c.append, no, no, [0], [100])          # fits: now the tensors
+    refused(lh.E_RANGE, c.read, [0], [0], [1])                   # nothing there yet
+    refused(lh.E_RANGE, c.read, [0], [-1], [0])
+    refused(lh.E_RANGE, c.attention, no, [0], [1])
+    refused(lh.E_INVALID, c.attention, no, [0], [0])
+    assert [c.length(s) for s in range(3)] == [0, 0, 0]
+
+
+def test_verify_refusals():
+    no = NoTensor()
+    refused(lh.E_INVALID, lh.verify_drafts, no, [1], [1], [0.5], [0.5])
+    refused(lh.E_INVALID, lh.verify_drafts, no, [1], [2], [0.5], [0.5])
+    refused(lh.E_INVALID, lh.verify_drafts, no, [1], [1], [0.5, 0.5], [0.5])
+    refused(lh.E_INVALID, lh.verify_drafts, no, [], [-1, 1], [], [0.5, 0.5])
+    accepted, tokens = lh.verify_drafts(no, [], [], [], [])
+    assert accepted.shape == (0,) and tokens.shape == (0, 1)
+
+
+def test_from_device_takes_device_memory_only():
+    refused(lh.E_INVALID, lh.Tensor.from_device, np.zeros(3, np.float32))
+
+    class Fake:
+        def __init__(self, **kw):
+            self.__cuda_array_interface__ = {"shape": (2, 3), "typestr": "<f4", "data": (0, False), "version": 3} | kw
+    refused(lh.E_DTYPE, lh.Tensor.from_device, Fake(typestr="<f2"))
+    refused(lh.E_INVALID, lh.Tensor.from_device, Fake(strides=(4, 8)))
