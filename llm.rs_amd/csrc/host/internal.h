@@ -79,6 +79,8 @@ struct Context {
   void* noalloc_scratch = nullptr;  // device address of the scratch on `device`
   std::string noalloc_error;        // why it is null
   uint8_t* host_out = nullptr;      // pinned: what fetch brings back (kFetchBytes + 64)
+  void* verify_tickets = nullptr;   // llmrs_verify_drafts: zero between calls
+  size_t n_verify_tickets = 0;
   std::vector<hipModule_t> modules;
   std::vector<std::string> module_names;
   std::map<std::string, KernelInfo> kernels;

@@ -18,6 +18,8 @@ struct llmrs_paged {
   std::vector<float> rope;       // cos, then sin; given back once on the device
   bool rotates = false;
   void *codes = nullptr, *exps = nullptr, *dtable = nullptr, *drope = nullptr;
+  void* tickets = nullptr;       // of split attention tiles, zero between launches
+  size_t n_tickets = 0;
 
   // Device memory, at the first call that needs it.
   void settle() {
@@ -41,11 +43,25 @@ struct llmrs_paged {
     rope.clear();
     rope.shrink_to_fit();
   }
+  int* zero_tickets(size_t n) {
+    if (n > n_tickets) {
+      Context& c = ctx();
+      if (tickets) c.alloc.release(tickets);
+      tickets = nullptr;
+      n_tickets = 0;
+      const size_t bytes = 2 * n * kTicketStride * sizeof(int);
+      tickets = c.alloc.alloc(bytes);
+      LLMRS_HIP(hipMemsetAsync(tickets, 0, bytes, c.stream));
+      n_tickets = 2 * n;
+    }
+    return (int*)tickets;
+  }
   void drop() {
-    for (void** p : {&codes, &exps, &dtable, &drope}) {
+    for (void** p : {&codes, &exps, &dtable, &drope, &tickets}) {
       if (*p) ctx().alloc.release(*p);
       *p = nullptr;
     }
+    n_tickets = 0;
   }
   int slot(int s, const char* what) const {
     LLMRS_REQUIRE(s >= 0 && s < cfg.max_seqs, LLMRS_E_RANGE,
@@ -145,20 +161,18 @@ void launch_rows(const llmrs_paged* p, const std::string& kernel, const std::vec
   launch(kernel + hd_tag(p), dim3((unsigned)a.seqs.items, (unsigned)p->cfg.n_kv_heads, 2), dim3(256), 0, ctx().stream, a);
 }
 
-// Columns (rows x query heads of a group) of a workgroup and how its four waves
-// share them: the narrowest that holds a sequence's columns, so that K and V are
-// read once.
+// Columns (rows x query heads of a group) of a workgroup, and the positions that it
+// takes at a time.
 struct AttnKind {
-  int waves, groups;  // waves across columns, groups of 16 columns per wave
-  int cols() const { return 16 * waves * groups; }
+  const char* name;
+  int cols, unit;
 };
-AttnKind attn_kind(int columns) {
-  return columns <= 16 ? AttnKind{1, 1} : columns <= 32 ? AttnKind{1, 2} : columns <= 64 ? AttnKind{2, 2} : AttnKind{4, 2};
-}
+constexpr AttnKind kFew{"few", 16, 256}, kMany1{"many1", 64, 64}, kMany2{"many2", 128, 64};
+AttnKind attn_kind(int columns) { return columns <= 16 ? kFew : columns <= 64 ? kMany1 : kMany2; }
 
-void launch_attention(const llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, const std::vector<Part>& parts,
+void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, const std::vector<Part>& parts,
                       AttnKind kind) {
-  const int nkv = p->cfg.n_kv_heads, hd = p->cfg.head_dim, cols = kind.cols();
+  const int nkv = p->cfg.n_kv_heads, hd = p->cfg.head_dim, cols = kind.cols;
   PagedAttnArgs a;
   a.pool = p->pool();
   a.q = (const float*)q->data;
@@ -167,12 +181,17 @@ void launch_attention(const llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor*
   a.rope_sin = p->sin();
   a.nq = (int)(q->dims[1] / (size_t)hd);
   a.scale = 1.0f / std::sqrt((float)hd);
-  const int n_rep = a.nq / nkv, unit = 64 * (4 / kind.waves);
+  const int n_rep = a.nq / nkv, unit = kind.unit;
   long units = 0;
   for (const Part& s : parts)
     units += (long)nkv * ((s.rows * n_rep + cols - 1) / cols) * ((s.pos + unit - 1) / unit);
-  const long want = 2 * ctx().num_cus;
-  a.chunk = (int)std::min<long>(((units + want - 1) / want) * unit, 1 << 24);
+  int longest = 0;
+  for (const Part& s : parts) longest = std::max(longest, s.pos);
+  static const char* env = std::getenv("PAGED_WANT");
+  const long want = (env ? std::atoi(env) : 2) * ctx().num_cus;
+  // units per split: enough workgroups, and no more splits than can be joined
+  const long per = std::max<long>((units + want - 1) / want, ((longest + unit - 1) / unit + kPagedMaxSplits - 1) / kPagedMaxSplits);
+  a.chunk = (int)std::min<long>(per * unit, 1 << 24);
   std::vector<int> items;
   bool split = false;
   for (const Part& s : parts) {
@@ -187,10 +206,9 @@ void launch_attention(const llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor*
   Scratch part(columns * 4 * (size_t)(hd + 2));
   a.part_o = (float*)part.p;
   a.part_ml = a.part_o ? a.part_o + columns * hd : nullptr;
+  a.tickets = split ? p->zero_tickets((size_t)a.seqs.items * nkv) : nullptr;
   const dim3 grid((unsigned)(a.seqs.items * nkv));
-  launch("paged_attn" + hd_tag(p) + "_c" + std::to_string(kind.waves) + "g" + std::to_string(kind.groups), grid, dim3(256), 0,
-         ctx().stream, a);
-  if (split) launch("paged_join" + hd_tag(p) + "_" + std::to_string(cols), grid, dim3(256), 0, ctx().stream, a);
+  launch("paged_attn" + hd_tag(p) + "_" + kind.name, grid, dim3(256), 0, ctx().stream, a);
 }
 
 }  // namespace

@@ -505,6 +505,7 @@ int llmrs_shutdown(void) {
   return guard([&] {
     if (!g_ctx) return;
     (void)hipStreamSynchronize(g_ctx->stream);
+    g_ctx->alloc.release(g_ctx->verify_tickets);
     g_ctx->alloc.trim();
     for (hipModule_t m : g_ctx->modules) (void)hipModuleUnload(m);
     (void)hipStreamDestroy(g_ctx->stream);

@@ -1,5 +1,6 @@
 // verify.cpp - llmrs_verify_drafts: drafted tokens against the target's
 // probabilities (verify.hip).
+#include <chrono>
 #include <cstring>
 
 #include "words.h"
@@ -12,6 +13,23 @@ void require_rows(const llmrs_tensor* t, size_t rows, size_t vocab, const char* 
   LLMRS_REQUIRE(t->dtype == LLMRS_F32, LLMRS_E_DTYPE, std::string("verify_drafts: ") + what + " must be an f32 tensor");
   LLMRS_REQUIRE(t->dims.size() == 2 && t->dims[0] == rows && t->dims[1] == vocab, LLMRS_E_INVALID,
                 std::string("verify_drafts: ") + what + " must be [" + std::to_string(rows) + ", " + std::to_string(vocab) + "]");
+}
+
+// Waits until every row starts with its stamp.  The kernel stores it last, so the
+// host sees it about 5 us before hipStreamSynchronize returns (an empty kernel,
+// launch to return: 6.6 against 11.5 us); work that is not done within a millisecond is
+// waited for there.
+void wait_for_stamps(const int* rows, size_t n, size_t row, int stamp) {
+  const auto until = std::chrono::steady_clock::now() + std::chrono::milliseconds(1);
+  for (size_t i = 0; i < n;) {
+    if (__atomic_load_n(rows + i * row, __ATOMIC_ACQUIRE) == stamp) ++i;
+    else if (std::chrono::steady_clock::now() > until) break;
+  }
+  for (size_t i = 0; i < n; ++i)
+    if (__atomic_load_n(rows + i * row, __ATOMIC_ACQUIRE) != stamp) {
+      LLMRS_HIP(hipStreamSynchronize(ctx().stream));
+      LLMRS_REQUIRE(__atomic_load_n(rows + i * row, __ATOMIC_ACQUIRE) == stamp, LLMRS_E_HIP, "verify_drafts: no answer");
+    }
 }
 
 }  // namespace
@@ -67,19 +85,45 @@ extern "C" int llmrs_verify_drafts(const llmrs_tensor* target, const llmrs_tenso
     a.groups = verify_groups((int)vocab);
     a.most = (int)most;
     a.drafts = (int)total;
-    const size_t row = 2 + most;
-    Scratch part(16 * n * (size_t)a.groups), out(4 * n * row);
+    const size_t row = 3 + most, bytes = 4 * n * row;
+    // tickets: zeroed here, and by each sequence's last workgroup
+    if (c.n_verify_tickets < n) {
+      if (c.verify_tickets) c.alloc.release(c.verify_tickets);
+      c.verify_tickets = nullptr;
+      c.n_verify_tickets = 0;
+      const size_t size = 2 * n * kTicketStride * sizeof(int);
+      c.verify_tickets = c.alloc.alloc(size);
+      LLMRS_HIP(hipMemsetAsync(c.verify_tickets, 0, size, c.stream));
+      c.n_verify_tickets = 2 * n;
+    }
+    const bool direct = bytes <= kFetchBytes;  // else through device memory
+    Scratch part(8 * n * (size_t)a.groups), out(direct ? 0 : bytes);
     a.part = (double*)part.p;
-    a.out = (int*)out.p;
+    a.tickets = (int*)c.verify_tickets;
+    a.out = direct ? (int*)c.host_out : (int*)out.p;
+    a.stamp = 1;
+    // slices per wave: as many as leave four workgroups per CU; each looks at all
+    // of its sequence's drafts first
+    const size_t groups4 = ((size_t)a.groups + 3) / 4;
+    a.per_wave = (int)std::max<size_t>(1, n * groups4 / (4 * (size_t)c.num_cus));
+    const unsigned grid = (unsigned)((groups4 + a.per_wave - 1) / a.per_wave);
+    if (direct)
+      for (size_t i = 0; i < n; ++i) __atomic_store_n((int*)c.host_out + i * row, 0, __ATOMIC_RELAXED);
     LaunchWords words(w, a.w);
     a.ext = words.ext();
-    launch("verify_sums", dim3((unsigned)a.groups, (unsigned)n), dim3(256), 0, c.stream, a);
-    launch("verify_pick", dim3((unsigned)n), dim3(256), 0, c.stream, a);
-    std::vector<int> got(n * row);
-    fetch(got.data(), out.p, 4 * got.size());
+    launch("verify_rows", dim3(grid, (unsigned)n), dim3(256), 0, c.stream, a);
+    std::vector<int> big;
+    const int* got = (const int*)c.host_out;
+    if (direct) {
+      wait_for_stamps((const int*)c.host_out, n, row, a.stamp);
+    } else {
+      big.resize(n * row);
+      fetch(big.data(), out.p, bytes);
+      got = big.data();
+    }
     for (size_t i = 0; i < n; ++i) {
-      accepted[i] = got[i * row];
-      for (size_t j = 0; j < width; ++j) tokens[i * width + j] = j <= most ? got[i * row + 1 + j] : -1;
+      accepted[i] = got[i * row + 1];
+      for (size_t j = 0; j < width; ++j) tokens[i * width + j] = j <= most ? got[i * row + 2 + j] : -1;
     }
   });
 }

@@ -510,12 +510,14 @@ struct PagedRowsArgs {
 
 // Attention of new rows.  A work item is a tile of (row, query head of the group)
 // columns and a split of `chunk` positions; items of one tile follow each other.
+constexpr int kPagedMaxSplits = 64;  // a lane each when they are joined
 struct PagedAttnArgs {
   PagedPool pool;
   const float* q;        // [rows][nq * hd]
   float* out;            // [rows][nq * hd]
   float* part_o;         // [item][KV head][columns][hd] (splits)
   float* part_ml;        // [item][KV head][columns][2]
+  int* tickets;          // [item][KV head][kTicketStride], zero between launches (a tile's first item counts)
   const float* rope_cos; // null: q as it is
   const float* rope_sin;
   int nq, chunk;
@@ -524,15 +526,18 @@ struct PagedAttnArgs {
 };
 
 // ---- verification of drafted tokens (verify.hip) -----------------------------
-constexpr int kVerifySlice = 2048;  // ids per workgroup
+constexpr int kVerifySlice = 512;  // ids of one sum (a wave's, 8 per lane)
 constexpr int kVerifyMaxDrafts = 64;
 constexpr int verify_groups(int vocab) { return (vocab + kVerifySlice - 1) / kVerifySlice; }
 struct VerifyArgs {
   const float* target;   // [rows][vocab]
   const float* draft;    // [drafted rows][vocab] (null: probability 1 at the drafted id)
-  double* part;          // [sequence][group][2] sums of a slice: what is left of the target, the target
-  int* out;              // [sequence][2 + most]: accepted, then its tokens (-1 past the last)
+  double* part;          // [sequence][group] sums of a slice
+  int* tickets;          // [sequence][kTicketStride], zero between launches
+  int* out;              // [sequence][3 + most]: stamp, accepted, its tokens (-1 past the last); the host's memory
   int vocab, n, groups, most;
+  int per_wave;          // slices of a wave
+  int stamp;             // what a finished row starts with
   // words (as PagedSeqs): per sequence its first target row, first drafted row and
   // drafts; then the drafted ids, their uniform numbers (f32 bits), the draws
   const int* ext;

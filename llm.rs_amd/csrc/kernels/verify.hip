@@ -18,7 +18,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / LLMRS_WAVE;
-constexpr int kPer = kVerifySlice / kThreads;  // ids per thread, consecutive
+constexpr int kPer = kVerifySlice / LLMRS_WAVE;  // ids per lane of a slice, consecutive
+constexpr int kHeld = 8;                         // sums of the slices, 64 at a time, that a wave holds
 
 __device__ __forceinline__ int word(const VerifyArgs& a, int i) { return a.ext ? a.ext[i] : a.w[i]; }
 
@@ -52,149 +53,194 @@ __device__ __forceinline__ Row examine(const VerifyArgs& a, int i) {
   return r;
 }
 
-// What is left of the target at id v, and the target (NaN counts as zero).
-__device__ __forceinline__ double weight(const Row& r, int v, double* target) {
-  const double p = r.p[v], q = r.q ? r.q[v] : v == r.drafted ? 1.0f : 0.0f;
-  *target = p > 0.0 ? p : 0.0;
-  const double w = p - q;
-  return w > 0.0 ? w : 0.0;
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any id
+
+// The weights of this thread's ids v0 .. v0 + 7: what is left of the target, or the
+// target itself; NaN counts as zero, ids past the vocabulary too.
+template <bool LEFT>
+__device__ __forceinline__ void weights(const VerifyArgs& a, const Row& r, int v0, double (&w)[kPer]) {
+  float p[kPer], q[kPer];
+  if (v0 + kPer <= a.vocab) {
+#pragma unroll
+    for (int k = 0; k < kPer; k += 4) {
+      const f32x4u x = *(const f32x4u*)(r.p + v0 + k);
+      f32x4u y = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (LEFT && r.q) y = *(const f32x4u*)(r.q + v0 + k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[k + i] = x[i];
+        q[k + i] = y[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      p[k] = v0 + k < a.vocab ? r.p[v0 + k] : 0.0f;
+      q[k] = LEFT && r.q && v0 + k < a.vocab ? r.q[v0 + k] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    if (LEFT && v0 + k == r.drafted) q[k] = 1.0f;
+    const double x = (double)p[k] - (LEFT ? (double)q[k] : 0.0);
+    w[k] = x > 0.0 ? x : 0.0;
+  }
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// Inclusive running sum over the lanes (row shifts, then the rows' last lanes
+// broadcast); lane 63 holds the total.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp64(double v) {
+  const dev_u32x2 u = __builtin_bit_cast(dev_u32x2, v);
+  const dev_u32x2 r = {(unsigned)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, ROWS, 0xF, false),
+                       (unsigned)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, ROWS, 0xF, false)};
+  return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double scan(double v) {
+  v += dpp64<0x111, 0xF>(v);  // row_shr:1, zero where the row begins
+  v += dpp64<0x112, 0xF>(v);
+  v += dpp64<0x114, 0xF>(v);
+  v += dpp64<0x118, 0xF>(v);
+  v += dpp64<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp64<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
+__device__ __forceinline__ double lane64(double v, int lane) {
+  const dev_u32x2 u = __builtin_bit_cast(dev_u32x2, v);
+  const dev_u32x2 r = {(unsigned)__builtin_amdgcn_readlane((int)u.x, lane), (unsigned)__builtin_amdgcn_readlane((int)u.y, lane)};
+  return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ int last_of(unsigned long long mask) { return 63 - __builtin_clzll(mask); }
 
-// Exclusive prefix over the workgroup's threads, and the total.
-__device__ double prefix(double v, double* red, double* total) {
-  double incl = v;
+// A slice's ids by one wave: the sum, and where the running sum from `base` exceeds
+// tau (-1: nowhere) and the last id that holds anything (-1: none).
+template <bool LEFT>
+__device__ __forceinline__ double slice_sum(const VerifyArgs& a, const Row& r, int slice, double (&w)[kPer]) {
+  weights<LEFT>(a, r, slice * kVerifySlice + lane_id() * kPer, w);
+  double sum = 0.0;
 #pragma unroll
-  for (int o = 1; o < LLMRS_WAVE; o <<= 1) {
-    const double t = __shfl_up(incl, o);
-    if (lane_id() >= o) incl += t;
-  }
-  if (lane_id() == LLMRS_WAVE - 1) red[wave_id()] = incl;
-  __syncthreads();
-  double base = 0.0, all = 0.0;
+  for (int k = 0; k < kPer; ++k) sum += w[k];
+  return scan(sum);
+}
+template <bool LEFT>
+__device__ __forceinline__ void slice_draw(const VerifyArgs& a, const Row& r, int slice, double base, double tau, int* id,
+                                           int* last) {
+  double w[kPer];
+  const double incl = slice_sum<LEFT>(a, r, slice, w);
+  double c = base + dpp64<0x138, 0xF>(incl);  // wave_shr:1: the lanes before
+  int hit = -1, top = -1;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave_id()) base += red[w];
-    all += red[w];
+  for (int k = 0; k < kPer; ++k) {
+    c += w[k];
+    if (w[k] > 0.0) {
+      top = k;
+      if (hit < 0 && c > tau) hit = k;
+    }
   }
-  __syncthreads();
-  *total = all;
-  return base + (incl - v);
+  const int v0 = slice * kVerifySlice;
+  const unsigned long long hits = __ballot(hit >= 0), tops = __ballot(top >= 0);
+  const int hl = hits ? __builtin_ctzll(hits) : 0, tl = tops ? last_of(tops) : 0;
+  *id = hits ? v0 + hl * kPer + __builtin_amdgcn_readlane(hit, hl) : -1;
+  *last = tops ? v0 + tl * kPer + __builtin_amdgcn_readlane(top, tl) : -1;
+}
+
+// The draw of a sequence, by one wave: `part` holds the slices' sums of what is
+// left of the target.
+__device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const unsigned* part, double u) {
+  const int lane = lane_id(), groups = a.groups;
+  double x[kHeld];  // running sums of 64 slices each
+  auto hold = [&](int g0) {
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) {
+      const int g = g0 + LLMRS_WAVE * c + lane;
+      x[c] = g < groups ? __builtin_bit_cast(double, dev_ld8(part, 8 * g)) : 0.0;
+    }
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) x[c] = scan(x[c]);
+  };
+  constexpr int HELD = LLMRS_WAVE * kHeld;
+  double total = 0.0;
+  for (int g0 = 0; g0 < groups; g0 += HELD) {
+    hold(g0);
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) total += lane64(x[c], 63);
+  }
+  int id = -1, last = -1;
+  if (!(total > 0.0)) {
+    // nothing is left of the target (rare): the target itself, slice by slice
+    double w[kPer];
+    for (int g = 0; g < groups; ++g) total += lane64(slice_sum<false>(a, r, g, w), 63);
+    const double tau = u * total;
+    double base = 0.0;
+    for (int g = 0; g < groups && id < 0; ++g) {
+      const double sum = lane64(slice_sum<false>(a, r, g, w), 63);
+      if (sum > 0.0) {
+        int top;
+        slice_draw<false>(a, r, g, base, tau, &id, &top);
+        last = top;
+      }
+      base += sum;
+    }
+    return id >= 0 ? id : last >= 0 ? last : a.vocab - 1;
+  }
+  // the first slice whose running sum exceeds tau, or the last that holds anything
+  const double tau = u * total;
+  double base = 0.0, from = 0.0;
+  int slice = -1, top = 0;
+  for (int g0 = 0; g0 < groups && slice < 0; g0 += HELD) {
+    if (groups > HELD) hold(g0);
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) {
+      const unsigned long long over = __ballot(base + x[c] > tau);
+      const double before = dpp64<0x138, 0xF>(x[c]);
+      const unsigned long long holds = __ballot(x[c] > before);
+      if (slice < 0 && over) {
+        const int l = __builtin_ctzll(over);
+        slice = g0 + LLMRS_WAVE * c + l;
+        from = base + lane64(before, l);
+      }
+      if (slice < 0 && holds) top = g0 + LLMRS_WAVE * c + last_of(holds);
+      base += lane64(x[c], 63);
+    }
+  }
+  // sums in another order may end just below what crossed: the slice's last id
+  if (slice >= 0) slice_draw<true>(a, r, slice, from, tau, &id, &last);
+  else slice_draw<true>(a, r, top, 0.0, INFINITY, &id, &last);
+  return id >= 0 ? id : last >= 0 ? last : a.vocab - 1;
 }
 
 }  // namespace
 
-// The sums of one slice of a sequence's row.
-extern "C" __global__ __launch_bounds__(kThreads) void verify_sums(VerifyArgs a) {
-  __shared__ double red[2][kWaves];
-  const int i = blockIdx.y, g = blockIdx.x;
+// A wave sums slices of a sequence's row.  The sequence's last workgroup (a ticket, no
+// waiting; the sums move with device-scope stores and loads) draws, one wave of it
+// alone: the slice in which the running sum crosses, and the id in that slice.  Its
+// answer goes straight to the host's memory, where the caller waits for the stamp that
+// follows it.
+extern "C" __global__ __launch_bounds__(kThreads) void verify_rows(VerifyArgs a) {
+  const int i = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(wave_id());
   const Row r = examine(a, i);
-  double left = 0.0, all = 0.0;
-  for (int v = g * kVerifySlice + threadIdx.x, n = 0; n < kPer; v += kThreads, ++n)
-    if (v < a.vocab) {
-      double t;
-      left += weight(r, v, &t);
-      all += t;
-    }
-  left = wave_sum64(left);
-  all = wave_sum64(all);
-  if (lane_id() == 0) {
-    red[0][wave_id()] = left;
-    red[1][wave_id()] = all;
+  unsigned* part = (unsigned*)(a.part + (size_t)i * a.groups);
+  const int first = blockIdx.x * kWaves * a.per_wave + wave, end = min(first + kWaves * a.per_wave, a.groups);
+  for (int g = first; g < end; g += kWaves) {
+    double w[kPer];
+    const double sum = slice_sum<true>(a, r, g, w);
+    if (lane_id() == 63) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(dev_u32x2, sum), dev_rsrc(part), 8 * g, 0, kSc1);
   }
+  __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double* dst = a.part + 2 * ((size_t)i * a.groups + g);
-    dst[0] = ((red[0][0] + red[0][1]) + red[0][2]) + red[0][3];
-    dst[1] = ((red[1][0] + red[1][1]) + red[1][2]) + red[1][3];
-  }
-}
-
-// The draw of one sequence: the slice that the running sum crosses in, then the id.
-extern "C" __global__ __launch_bounds__(kThreads) void verify_pick(VerifyArgs a) {
-  __shared__ double red[kWaves];
-  __shared__ int found, last;
-  __shared__ double before;
-  const int i = blockIdx.x, tid = threadIdx.x;
-  const Row r = examine(a, i);
-  const double* part = a.part + 2 * (size_t)i * a.groups;
-  const double u = __int_as_float(word(a, 3 * a.n + 2 * a.drafts + i));
-  // groups in index order, consecutive ones per thread
-  const int per = (a.groups + kThreads - 1) / kThreads;
-  const int g0 = min(a.groups, tid * per), g1 = min(a.groups, g0 + per);
-  double mine = 0.0, total;
-  for (int g = g0; g < g1; ++g) mine += part[2 * g];
-  double base = prefix(mine, red, &total);
-  const int which = total > 0.0 ? 0 : 1;
-  if (which) {
-    mine = 0.0;
-    for (int g = g0; g < g1; ++g) mine += part[2 * g + 1];
-    base = prefix(mine, red, &total);
-  }
-  const double tau = u * total;
-  if (tid == 0) {
-    found = 0x7FFFFFFF;
-    last = -1;
-  }
-  __syncthreads();
-  int hit = -1;
-  double hit_base = 0.0;
-  for (int g = g0; g < g1; ++g) {
-    const double w = part[2 * g + which];
-    if (hit < 0 && base + w > tau) {
-      hit = g;
-      hit_base = base;
-    }
-    if (w > 0.0) atomicMax(&last, g);
-    base += w;
-  }
-  if (hit >= 0) atomicMin(&found, hit);
-  __syncthreads();
-  // no slice crosses (rounding): the last one that holds anything
-  const int group = found != 0x7FFFFFFF ? found : last;
-  if (hit == group && hit >= 0) before = hit_base;
-  __syncthreads();
-  const bool end = found == 0x7FFFFFFF;
-  const double from = end ? 0.0 : before;
-  __syncthreads();
-  if (tid == 0) {
-    found = 0x7FFFFFFF;
-    last = -1;
-  }
-  __syncthreads();
-  if (group >= 0) {
-    const int v0 = group * kVerifySlice + tid * kPer;
-    double w[kPer], sum = 0.0, all;
-#pragma unroll
-    for (int n = 0; n < kPer; ++n) {
-      double t = 0.0, l = 0.0;
-      if (v0 + n < a.vocab) l = weight(r, v0 + n, &t);
-      w[n] = which ? t : l;
-      sum += w[n];
-    }
-    double c = from + prefix(sum, red, &all);
-    int id = -1, top = -1;
-#pragma unroll
-    for (int n = 0; n < kPer; ++n) {
-      c += w[n];
-      if (w[n] > 0.0) {
-        top = v0 + n;
-        if (id < 0 && !end && c > tau) id = v0 + n;
-      }
-    }
-    if (id >= 0) atomicMin(&found, id);
-    if (top >= 0) atomicMax(&last, top);
-  }
-  __syncthreads();
-  // the running sum of one order may end just below what another crossed: the last id
-  const int drawn = found != 0x7FFFFFFF ? found : last >= 0 ? last : a.vocab - 1;
-  int* out = a.out + (size_t)i * (a.most + 2);
-  if (tid == 0) out[0] = r.accepted;
-  for (int j = tid; j <= a.most; j += kThreads)
-    out[1 + j] = j < r.accepted ? word(a, 3 * a.n + r.first + j) : j == r.accepted ? drawn : -1;
+  if (wave) return;
+  int ticket = 0;
+  if (tid == 0) ticket = atomicAdd(a.tickets + (size_t)i * kTicketStride, 1);
+  if (__builtin_amdgcn_readfirstlane(ticket) != (int)gridDim.x - 1) return;
+  if (tid == 0) dev_stu(a.tickets + (size_t)i * kTicketStride, 0, 0u);  // as it was found, for the next launch
+  const int drawn = draw(a, r, part, __int_as_float(word(a, 3 * a.n + 2 * a.drafts + i)));
+  // words to the host's memory, each written through; the stamp once they are there
+  int* out = a.out + (size_t)i * (a.most + 3);
+  auto put = [](int* at, int v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); };
+  if (tid == 0) put(out + 1, r.accepted);
+  for (int j = tid; j <= a.most; j += LLMRS_WAVE)
+    put(out + 2 + j, j < r.accepted ? word(a, 3 * a.n + r.first + j) : j == r.accepted ? drawn : -1);
+  __builtin_amdgcn_s_waitcnt(0);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  if (tid == 0) put(out, a.stamp);
 }

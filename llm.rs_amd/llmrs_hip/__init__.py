@@ -226,13 +226,25 @@ def num_cus() -> int:
     return lib().llmrs_num_cus()
 
 
+def _ref(a: np.ndarray):
+    """A contiguous array as an argument: its buffer by reference, several times
+    cheaper than ndarray.ctypes (read-only arrays take that way)."""
+    if not a.size:
+        return None
+    try:
+        return C.byref(C.c_char.from_buffer(a))
+    except TypeError:
+        return a.ctypes.data
+
+
 class Tensor:
     """A device tensor handle (Tensor with Storage on Device::Hip)."""
 
-    __slots__ = ("_h", "__weakref__")
+    __slots__ = ("_h", "_shape", "__weakref__")
 
-    def __init__(self, handle: int):
-        self._h = C.c_void_p(handle)
+    def __init__(self, handle, shape: tuple[int, ...] | None = None):
+        self._h = handle if isinstance(handle, C.c_void_p) else C.c_void_p(handle)
+        self._shape = shape  # None: asked for when it is needed
 
     @property
     def handle(self):
@@ -240,10 +252,12 @@ class Tensor:
 
     @property
     def shape(self) -> tuple[int, ...]:
-        nd = _check(lib().llmrs_tensor_ndim(self._h))
-        dims = (C.c_size_t * nd)()
-        _check(lib().llmrs_tensor_dims(self._h, dims))
-        return tuple(int(d) for d in dims)
+        if self._shape is None:
+            nd = _check(lib().llmrs_tensor_ndim(self._h))
+            dims = (C.c_size_t * nd)()
+            _check(lib().llmrs_tensor_dims(self._h, dims))
+            self._shape = tuple(int(d) for d in dims)
+        return self._shape
 
     @property
     def dtype(self) -> DType:
@@ -301,9 +315,8 @@ class Tensor:
         """An f32 tensor's values in place, for another library in this
         process: while this object lives, and not before ``sync()`` where
         work on them is still queued."""
-        at = C.c_void_p()
+        at, shape = C.c_void_p(), self.shape
         _check(lib().llmrs_tensor_address(self._h, C.byref(at)))
-        shape = self.shape
         return {"shape": shape, "typestr": "<f4", "data": (0 if 0 in shape else at.value, False), "version": 3}
 
     @staticmethod
@@ -741,12 +754,18 @@ class PagedConfig(C.Structure):
                 ("max_seqs", C.c_int32), ("max_seq", C.c_int32), ("rope_theta", C.c_float)]
 
 
-def _i32(a) -> np.ndarray:
-    return np.ascontiguousarray(a, dtype=np.int32).reshape(-1)
+def _vec(a, dtype) -> np.ndarray:
+    """A flat contiguous array; one that is, as it is."""
+    if type(a) is np.ndarray and a.dtype is dtype and a.ndim == 1 and a.flags.c_contiguous:
+        return a
+    return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
+
+
+_I32, _F32 = np.dtype(np.int32), np.dtype(np.float32)
 
 
 def _pair(a, b, what: str):
-    a, b = _i32(a), _i32(b)
+    a, b = _vec(a, _I32), _vec(b, _I32)
     if a.size != b.size:
         raise LlmrsError(E_INVALID, f"{what}: {a.size} slots, {b.size} numbers")
     return a, b
@@ -766,6 +785,7 @@ class HipPagedCache:
                 raise LlmrsError(E_INVALID, "rope tables must be [max_seq][head_dim/2]")
         elif rope is not None:
             theta = float(rope)
+        self._width = n_kv_heads * head_dim
         self.cfg = PagedConfig(n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_seq, theta)
         h = C.c_void_p()
         _check(lib().llmrs_paged_create(C.byref(self.cfg), _ptr(cos), _ptr(sin), C.byref(h)))
@@ -784,8 +804,8 @@ class HipPagedCache:
 
     def map(self, slot: int, pages) -> None:
         """Adds pages at the end of a slot's."""
-        pages = _i32(pages)
-        _check(lib().llmrs_paged_map(self._h, int(slot), _ptr(pages), pages.size))
+        pages = _vec(pages, _I32)
+        _check(lib().llmrs_paged_map(self._h, int(slot), _ref(pages), pages.size))
 
     def release(self, slot: int) -> None:
         """Ends a slot's sequence and frees its pages."""
@@ -799,42 +819,45 @@ class HipPagedCache:
     def truncate(self, slots, lengths) -> None:
         """Shortens sequences to the given lengths."""
         slots, lengths = _pair(slots, lengths, "truncate")
-        _check(lib().llmrs_paged_truncate(self._h, _ptr(slots), _ptr(lengths), slots.size))
+        _check(lib().llmrs_paged_truncate(self._h, _ref(slots), _ref(lengths), slots.size))
 
     def append(self, k: Tensor, v: Tensor, slots, counts, rotate: bool = True) -> None:
         """Appends counts[i] rows of k and v to slots[i], k rotated to its
         positions on the way (rotate=False: it is already)."""
         slots, counts = _pair(slots, counts, "append")
-        _check(lib().llmrs_paged_append(self._h, k.handle, v.handle, _ptr(slots), _ptr(counts), slots.size,
-                                        1 if rotate else 0))
+        _check(lib().llmrs_paged_append(self._h, k.handle, v.handle, _ref(slots), _ref(counts), slots.size, 1 if rotate else 0))
 
     def read(self, slots, starts, counts) -> tuple[Tensor, Tensor]:
         """Rows [starts[i], starts[i] + counts[i]) of slots[i] as f32: (K, V)."""
         slots, counts = _pair(slots, counts, "read")
         slots, starts = _pair(slots, starts, "read")
         k, v = C.c_void_p(), C.c_void_p()
-        _check(lib().llmrs_paged_read(self._h, _ptr(slots), _ptr(starts), _ptr(counts), slots.size, C.byref(k), C.byref(v)))
-        return Tensor(k.value), Tensor(v.value)
+        _check(lib().llmrs_paged_read(self._h, _ref(slots), _ref(starts), _ref(counts), slots.size, C.byref(k), C.byref(v)))
+        shape = (sum(counts.tolist()), self._width)
+        return Tensor(k, shape), Tensor(v, shape)
 
     def attention(self, q: Tensor, slots, counts) -> Tensor:
         """Causal attention of the last counts[i] positions of slots[i] (already
         appended); q is rotated on the way."""
         slots, counts = _pair(slots, counts, "attention")
-        return _out_tensor(lib().llmrs_paged_attention, self._h, q.handle, _ptr(slots), _ptr(counts), slots.size)
+        out = C.c_void_p()
+        _check(lib().llmrs_paged_attention(self._h, q.handle, _ref(slots), _ref(counts), slots.size, C.byref(out)))
+        return Tensor(out, q.shape)
 
 
 def verify_drafts(target: Tensor, ids, counts, accept, draw, draft: Tensor | None = None) -> tuple[np.ndarray, np.ndarray]:
     """Drafted tokens against the target's probabilities, from given uniform
     numbers (llmrs_verify_drafts): accepted drafts per sequence, and their ids
     followed by the next token's, -1 past it."""
-    ids, counts = _i32(ids), _i32(counts)
-    accept, draw = (np.ascontiguousarray(a, dtype=np.float32).reshape(-1) for a in (accept, draw))
-    if counts.size and counts.min() < 0 or ids.size != counts.sum() or accept.size != ids.size or draw.size != counts.size:
+    ids, counts, accept, draw = _vec(ids, _I32), _vec(counts, _I32), _vec(accept, _F32), _vec(draw, _F32)
+    each = counts.tolist()
+    if min(each, default=0) < 0 or ids.size != sum(each) or accept.size != ids.size or draw.size != counts.size:
         raise LlmrsError(E_INVALID, "verify_drafts: one id and one number per draft, one draw per sequence")
-    width = int(counts.max()) + 1 if counts.size else 1
+    width = max(each, default=0) + 1
     accepted, tokens = np.empty(counts.size, np.int32), np.empty((counts.size, width), np.int32)
-    _check(lib().llmrs_verify_drafts(target.handle, draft.handle if draft is not None else None, _ptr(ids), _ptr(counts),
-                                     _ptr(accept), _ptr(draw), counts.size, _ptr(accepted), _ptr(tokens), width))
+    _check(lib().llmrs_verify_drafts(target.handle, draft.handle if draft is not None else None,
+                                     _ref(ids), _ref(counts), _ref(accept), _ref(draw), counts.size, _ref(accepted),
+                                     _ref(tokens), width))
     return accepted, tokens
 
 
