@@ -161,14 +161,43 @@ void launch_rows(const llmrs_paged* p, const std::string& kernel, const std::vec
   launch(kernel + hd_tag(p), dim3((unsigned)a.seqs.items, (unsigned)p->cfg.n_kv_heads, 2), dim3(256), 0, ctx().stream, a);
 }
 
-// Columns (rows x query heads of a group) of a workgroup, and the positions that it
-// takes at a time.
+// A kernel's columns per workgroup and the positions that its waves take at a time.
 struct AttnKind {
   const char* name;
   int cols, unit;
 };
-constexpr AttnKind kFew{"few", 16, 256}, kMany1{"many1", 64, 64}, kMany2{"many2", 128, 64};
-AttnKind attn_kind(int columns) { return columns <= 16 ? kFew : columns <= 64 ? kMany1 : kMany2; }
+constexpr AttnKind kFew{"few", 16, 256}, kMany{"many", 64, 64};
+// Columns per CU from which the kernel of 64 is the faster: with 64 of them (512 rows
+// of 32 heads behind 500 positions) 29.3 us against 27.4, with 100 (4 x 200 rows
+// behind 1000) 36.1 against 39.3, with 128 45.2 against 46.9, with 256 (4 x 512 rows) 29.5
+// against 55.2 and with 256 behind 2048 positions 194 against 277.
+constexpr long kManyColumns = 96;
+
+// Units of a split.  One workgroup per CU: a second one has each wait for the other's
+// loads, and doubles what is joined (8 sequences of 4000 positions: 16.7 us either way;
+// one of 2048 with 32 columns a head 13.8 us with one, 16.3 with two).  Where that
+// would split nothing though CUs stand half empty behind long caches, two (16
+// sequences of 2100, two workgroups a head: 19.5 us against 23.8).  A batch that fills
+// the chip unsplit keeps whole sequences but for the ones that would outlast it.
+int split_units(const std::vector<Part>& parts, long heads, int n_rep, const AttnKind& kind, long cus) {
+  long units = 0, whole = 0;
+  int longest = 0;
+  auto tiles = [&](const Part& s) { return heads * ((s.rows * (long)n_rep + kind.cols - 1) / kind.cols); };
+  for (const Part& s : parts) {
+    units += tiles(s) * ((s.pos + kind.unit - 1) / kind.unit);
+    whole += tiles(s);
+    longest = std::max(longest, s.pos);
+  }
+  const long slots = 2 * whole > cus && whole <= cus ? 2 * cus : cus;
+  const int most = (longest + kind.unit - 1) / kind.unit;
+  int per = (int)std::max<long>((units + slots - 1) / slots, (most + kPagedMaxSplits - 1) / kPagedMaxSplits);
+  for (; whole <= slots && per < most; ++per) {
+    long groups = 0;
+    for (const Part& s : parts) groups += tiles(s) * ((s.pos + per * kind.unit - 1) / (per * kind.unit));
+    if (groups <= slots) break;
+  }
+  return std::min(per, most);
+}
 
 void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, const std::vector<Part>& parts,
                       AttnKind kind) {
@@ -182,16 +211,8 @@ void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, 
   a.nq = (int)(q->dims[1] / (size_t)hd);
   a.scale = 1.0f / std::sqrt((float)hd);
   const int n_rep = a.nq / nkv, unit = kind.unit;
-  long units = 0;
-  for (const Part& s : parts)
-    units += (long)nkv * ((s.rows * n_rep + cols - 1) / cols) * ((s.pos + unit - 1) / unit);
-  int longest = 0;
-  for (const Part& s : parts) longest = std::max(longest, s.pos);
-  static const char* env = std::getenv("PAGED_WANT");
-  const long want = (env ? std::atoi(env) : 2) * ctx().num_cus;
-  // units per split: enough workgroups, and no more splits than can be joined
-  const long per = std::max<long>((units + want - 1) / want, ((longest + unit - 1) / unit + kPagedMaxSplits - 1) / kPagedMaxSplits);
-  a.chunk = (int)std::min<long>(per * unit, 1 << 24);
+  const int per = split_units(parts, nkv, n_rep, kind, ctx().num_cus);
+  a.chunk = per * unit;
   std::vector<int> items;
   bool split = false;
   for (const Part& s : parts) {
@@ -202,13 +223,14 @@ void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, 
   a.seqs.n = (int)parts.size();
   const LaunchWords words(seq_words(parts, items, &a.seqs.items), a.seqs.w);
   a.seqs.ext = words.ext();
+  LLMRS_REQUIRE((long)a.seqs.items * nkv < (1L << 31), LLMRS_E_INVALID, "paged_attention: too much work for one call");
   const size_t columns = split ? (size_t)a.seqs.items * nkv * cols : 0;
   Scratch part(columns * 4 * (size_t)(hd + 2));
   a.part_o = (float*)part.p;
   a.part_ml = a.part_o ? a.part_o + columns * hd : nullptr;
   a.tickets = split ? p->zero_tickets((size_t)a.seqs.items * nkv) : nullptr;
   const dim3 grid((unsigned)(a.seqs.items * nkv));
-  launch("paged_attn" + hd_tag(p) + "_" + kind.name, grid, dim3(256), 0, ctx().stream, a);
+  launch(std::string("paged_attn_") + kind.name + hd_tag(p), grid, dim3(256), 0, ctx().stream, a);
 }
 
 }  // namespace
@@ -390,20 +412,20 @@ int llmrs_paged_attention(llmrs_paged* p, const llmrs_tensor* q, const int32_t* 
     (void)ctx();
     OnDevice here;
     Rows o(new_rows(rows, q->dims[1]));
-    // short and long column counts in launches of their own: a prompt among
-    // decoding sequences leaves these their narrow kernels
-    const int n_rep = (int)(q->dims[1] / group);
+    // The kernel of 64 columns reads a cache a quarter as often, but needs columns for
+    // every CU's waves; sequences that do not fill one of its workgroups stay with the
+    // kernel of 16.
+    const long n_rep = (long)(q->dims[1] / group);
     std::vector<Part> few, many;
-    int most = 0;
+    long columns = 0;
     for (const Part& s : parts) {
-      if ((long)s.rows * n_rep > 64) many.push_back(s);
-      else {
-        few.push_back(s);
-        most = std::max(most, s.rows * n_rep);
-      }
+      const bool fills = s.rows * n_rep >= kMany.cols;
+      (fills ? many : few).push_back(s);
+      if (fills) columns += s.rows * n_rep * p->cfg.n_kv_heads;
     }
-    if (!few.empty()) launch_attention(p, q, o.get(), few, attn_kind(most));
-    if (!many.empty()) launch_attention(p, q, o.get(), many, attn_kind(65));
+    if (columns < kManyColumns * ctx().num_cus) few = parts, many.clear();
+    if (!few.empty()) launch_attention(p, q, o.get(), few, kFew);
+    if (!many.empty()) launch_attention(p, q, o.get(), many, kMany);
     *out = o.release();
   });
 }

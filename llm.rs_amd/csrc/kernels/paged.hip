@@ -35,13 +35,16 @@ struct Seq {
 // The sequence of a work item: the last one whose first item is not past it
 // (a sequence without items starts where the next one does).
 __device__ __forceinline__ Seq find_seq(const PagedSeqs& s, int item) {
+  // one value per wave, and so held in scalar registers: the compiler takes what is
+  // loaded from either of two places to differ from lane to lane
+  auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   Seq q;
   if (s.n == 1) {
     q.item = item;
-    q.slot = s.w[1];
-    q.row0 = s.w[2];
-    q.rows = s.w[3];
-    q.pos = s.w[4];
+    q.slot = uni(s.w[1]);
+    q.row0 = uni(s.w[2]);
+    q.rows = uni(s.w[3]);
+    q.pos = uni(s.w[4]);
     return q;
   }
   int i = -1;
@@ -49,19 +52,19 @@ __device__ __forceinline__ Seq find_seq(const PagedSeqs& s, int item) {
     const int l = b + lane_id();
     i += __popcll(__ballot(l < s.n && word(s, l < s.n ? l : 0) <= item));
   }
-  i = __builtin_amdgcn_readfirstlane(i);
+  i = uni(i);
   const int at = s.n + 4 * i;
-  q.item = item - word(s, i);
-  q.slot = word(s, at);
-  q.row0 = word(s, at + 1);
-  q.rows = word(s, at + 2);
-  q.pos = word(s, at + 3);
+  q.item = item - uni(word(s, i));
+  q.slot = uni(word(s, at));
+  q.row0 = uni(word(s, at + 1));
+  q.rows = uni(word(s, at + 2));
+  q.pos = uni(word(s, at + 3));
   return q;
 }
 
 // The pool block that holds block `b` of a slot.
 __device__ __forceinline__ int pool_block(const PagedPool& p, int slot, int b) {
-  return (p.table[(size_t)slot * p.stride + (b >> p.shift)] << p.shift) + (b & ((1 << p.shift) - 1));
+  return (__builtin_amdgcn_readfirstlane(p.table[(size_t)slot * p.stride + (b >> p.shift)]) << p.shift) + (b & ((1 << p.shift) - 1));
 }
 
 // The smallest e in [kPagedExpMin, kPagedExpMax] with amax <= 127 * 2^e: amax =
@@ -208,8 +211,9 @@ extern "C" __global__ __launch_bounds__(kThreads) void paged_read_hd128(PagedRow
 //   S^T = K Q^T    v_mfma_i32_16x16x64_i8: the K codes are the operand as they
 //                  lie in the cache; q is a fixed-point number of 22 bits below
 //                  its largest magnitude, in three signed bytes, so the sums are
-//                  exact and a score is off by the rounding of q (2^-23 of its
-//                  largest value) and of two f32 operations.
+//                  exact; a score is off by the rounding of q (2^-23 of its
+//                  largest value), by less than a step of 2^-14 of it and the
+//                  block's, and by two f32 roundings.
 //   softmax        online per column, exp2 of log2(e)-scaled scores.
 //   O^T += V^T P^T v_mfma_f32_16x16x32_f16: the V codes as f16 (a byte placed in
 //                  1024 + code + 128, less 1152), p times the block's scale as f16
@@ -219,6 +223,7 @@ extern "C" __global__ __launch_bounds__(kThreads) void paged_read_hd128(PagedRow
 // Lane l of a tile: column c = l % 16, positions 16 (l / 16) .. + 15, all in one
 // block, so both exponents are a lane's own.
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNone = -1e30f;
 
 // One value of q in fixed point: n = n2 2^16 + n1 2^8 + n0, three signed bytes, byte
 // `b` of a word each.
@@ -235,11 +240,12 @@ __device__ __forceinline__ int row_exp(float amax, bool odd) {
   return amax > 0.0f && !odd ? 22 - __builtin_amdgcn_frexp_expf(amax) : 0;
 }
 __device__ __forceinline__ float row_scale(float scale, int ex, bool odd) {
-  return odd ? NAN : ldexpf(scale * kLog2e, -ex);
+  return odd ? NAN : ldexpf(scale * kLog2e, 8 - ex);  // scores come in steps of 2^8
 }
 
 // Eight codes of V (positions of one half of a lane's 16) as f16.
 __device__ __forceinline__ h16x8 v_half(unsigned w0, unsigned w1) {
+  asm("" : "+v"(w0), "+v"(w1));  // words: else the compiler carries them to here byte by byte
   const h16x2 less = {(_Float16)-1152.0f, (_Float16)-1152.0f};
   h16x8 v;
 #pragma unroll
@@ -255,87 +261,124 @@ __device__ __forceinline__ h16x8 v_half(unsigned w0, unsigned w1) {
   return v;
 }
 
+// What two weights have over their f16 parts, rounded to f16: the mixed-precision
+// operation takes the f16 as it is (exact: hi * -1 + w).
+__device__ __forceinline__ h16x2 rest(h16x2 hi, float w0, float w1) {
+  const unsigned h = __builtin_bit_cast(unsigned, hi);
+  float a, b;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(h), "v"(w0));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(h), "v"(w1));
+  return h16x2{(_Float16)a, (_Float16)b};
+}
+
+// Two maxima over the lanes that share l % 16.  The exchanges of halves and rows
+// take two values at once.
+__device__ __forceinline__ void max_groups(float& x, float& y) {
+  auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  float v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));  // lower half: x, upper half: y
+  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  x = __uint_as_float(p[0]);
+  y = __uint_as_float(p[1]);
+}
+
 // The running state of a wave's 16 columns.
 template <int HD>
 struct Column {
-  float m = -INFINITY, mw = -INFINITY, l = 0.0f;  // l: of this lane's positions
+  // before a column has seen a position, its maxima are far below every score's, and
+  // finite, so that the exponents' differences are numbers
+  float m = kNone, mw = kNone, l = 0.0f;  // l: of this lane's positions
+  float oc = 1.0f;
+  bool grown = false;
   f32x4 o[HD / 16];                               // 2^(14 - mw) O: dims 16 d + 4 r + i
   __device__ __forceinline__ Column() {
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // Scores of a tile (not yet scaled) from the integer sums, and their maximum.
-  // past: the column's last visible position less the lane's first.
-  template <class K, class Q>
-  static __device__ __forceinline__ float scores(K&& k, Q&& q, bool cut, int past, float (&sv)[16]) {
-    float mx = -INFINITY;
+  // Scores of a tile (not yet scaled) from the integer sums: the lowest bytes' sum
+  // enters in whole steps of 2^8, rounded down like every other's, as what the next
+  // bytes' sum starts from.
+  template <int BH, class K, class Q>
+  static __device__ __forceinline__ void scores(K&& k, Q&& q, float (&sv)[16]) {
+    // BH operand rows at a time: their chains are independent of each other
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      i32x4 s2 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0}, s0 = {0, 0, 0, 0};
+    for (int b0 = 0; b0 < 4; b0 += BH) {
+      i32x4 hi[BH], lo[BH];
 #pragma unroll
-      for (int s = 0; s < HD / 64; ++s) {
-        const i32x4 x = k(b, s);
-        s2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, q(2, s), s2, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, q(1, s), s1, 0, 0, 0);
-        s0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, q(0, s), s0, 0, 0, 0);
-      }
+      for (int b = 0; b < BH; ++b) lo[b] = hi[b] = i32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = __builtin_fmaf((float)((s2[i] << 8) + s1[i]), 256.0f, (float)s0[i]);
-        if (cut && 4 * b + i > past) x = -INFINITY;
-        sv[4 * b + i] = x;
-        mx = fmaxf(mx, x);
-      }
+      for (int s = 0; s < HD / 64; ++s)
+#pragma unroll
+        for (int b = 0; b < BH; ++b) lo[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k(b0 + b, s), q(0, s), lo[b], 0, 0, 0);
+#pragma unroll
+      for (int s = 0; s < HD / 64; ++s)
+#pragma unroll
+        for (int b = 0; b < BH; ++b) hi[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k(b0 + b, s), q(2, s), hi[b], 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < BH; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lo[b][i] >>= 8;
+#pragma unroll
+      for (int s = 0; s < HD / 64; ++s)
+#pragma unroll
+        for (int b = 0; b < BH; ++b) lo[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k(b0 + b, s), q(1, s), lo[b], 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < BH; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sv[4 * (b0 + b) + i] = (float)((hi[b][i] << 8) + lo[b][i]);
     }
-    return mx;
+  }
+
+  // Positions that the column does not see: e > past.
+  static __device__ __forceinline__ void hide(int past, float (&sv)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sv[e] = e > past ? -INFINITY : sv[e];
   }
 
   // Weights of a tile as f16 hi + lo; the state moves to the new maxima.
-  __device__ __forceinline__ void weigh(const float (&sv)[16], float mx, float sl2, int ek, float ev, h16x8 (&ph)[2],
-                                        h16x8 (&pl)[2]) {
+  __device__ __forceinline__ void weigh(const float (&sv)[16], float sl2, int ek, float ev, h16x8 (&ph)[2], h16x8 (&pl)[2]) {
+    float mx = sv[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sv[e]);
     // the scale of q and the block: kept above zero, so that a position out of
     // sight stays at -inf (NaN is kept)
     float f = ldexpf(sl2, ek);
     f = f < 1e-38f ? 1e-38f : f;
     mx = mx * f;
     float mb = mx + ev;
-    mx = fmaxf(mx, xor16(mx));
-    mb = fmaxf(mb, xor16(mb));
-    mx = fmaxf(mx, xor32(mx));
-    mb = fmaxf(mb, xor32(mb));
+    max_groups(mx, mb);
     const float mn = fmaxf(m, mx), wn = fmaxf(mw, mb);
-    const float at = mn == -INFINITY ? 0.0f : mn;  // no position seen yet: every p is 2^-inf
-    const float wt = wn == -INFINITY ? 0.0f : wn;
-    l *= __builtin_amdgcn_exp2f(m - at);
-    const float oc = __builtin_amdgcn_exp2f(mw - wt);
-    // 2^14 puts the weights' hi and lo parts in f16's range
-    const float gain = __builtin_amdgcn_exp2f(fminf(ev + at - wt, 100.0f) + 14.0f);
+    // a weight is p 2^gain: 2^14 puts hi and lo in f16's range, and below 2^-30 both are
+    // zero whatever the gain, while p still counts in the sum
+    const float gain = fmaxf(ev + (mn - wn) + 14.0f, -30.0f), less = gain - mn;
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], f, -at));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], f, -at));
-      sum += p0;
-      sum += p1;
-      float w0 = p0 * gain, w1 = p1 * gain;
-      // hi has to be the rounded product's: unhindered, the compiler rounds
-      // the exact one to f16 for the operand and this one for lo, an f16 step apart
-      // where they fall on two sides of a tie
-      asm("" : "+v"(w0), "+v"(w1));
+      const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], f, less));
+      const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], f, less));
+      sum += w0;
+      sum += w1;
       const h16x2 hi = __builtin_bit_cast(h16x2, __builtin_amdgcn_cvt_pkrtz(w0, w1));
+      const h16x2 lo = rest(hi, w0, w1);
       ph[e >> 3][e & 7] = hi.x;
       ph[e >> 3][(e & 7) + 1] = hi.y;
-      pl[e >> 3][e & 7] = (_Float16)(w0 - (float)hi.x);
-      pl[e >> 3][(e & 7) + 1] = (_Float16)(w1 - (float)hi.y);
+      pl[e >> 3][e & 7] = lo.x;
+      pl[e >> 3][(e & 7) + 1] = lo.y;
     }
-    l += sum;
-    if (__ballot(wn != mw)) {
+    l = l * __builtin_amdgcn_exp2f(m - mn) + sum * __builtin_amdgcn_exp2f(-gain);
+    m = mn;
+    grown = __ballot(wn != mw) != 0;
+    oc = __builtin_amdgcn_exp2f(mw - wn);
+    mw = wn;
+  }
+  // O to the new maximum, where a column's has risen.
+  __device__ __forceinline__ void rescale() {
+    if (grown) {
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) o[d] = o[d] * oc;
     }
-    m = mn;
-    mw = wn;
   }
 
   // The lanes' sums together, and O as the weighted mean of V.
@@ -365,6 +408,7 @@ __device__ __forceinline__ Item item_of(const PagedAttnArgs& a, int cols) {
   t.n_split = (t.q.pos + a.chunk - 1) / a.chunk;
   t.tile = t.q.item / t.n_split;
   t.split = t.q.item % t.n_split;
+  t.tile = (t.n_col + cols - 1) / cols - 1 - t.tile;  // the last rows see the most: they come first
   // up to the last position that any of the tile's columns sees
   t.from = t.split * a.chunk;
   t.to = min(t.from + a.chunk, t.past + (min((t.tile + 1) * cols, t.n_col) - 1) / t.n_rep + 1);
@@ -398,67 +442,103 @@ __device__ __forceinline__ void put_column(const PagedAttnArgs& a, const Item& t
   const size_t unit = ((size_t)t.item * a.pool.nkv + t.head) * cols;
 #pragma unroll
   for (int d = 0; d < HD / 16; ++d)
-    dev_st16(a.part_o + unit * HD, (local * HD + 16 * d + 4 * r) * 4, __builtin_bit_cast(dev_u32x4, x.o[d]));
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(dev_u32x4, x.o[d]), dev_rsrc(a.part_o + unit * HD),
+                                           (local * HD + 16 * d + 4 * r) * 4, 0, kSc1);
   if (r == 0) {
-    dev_stf(a.part_ml + unit * 2, local * 8, x.m);
-    dev_stf(a.part_ml + unit * 2, local * 8 + 4, x.l);
+    __builtin_amdgcn_raw_buffer_store_b64(dev_u32x2{__float_as_uint(x.m), __float_as_uint(x.l)}, dev_rsrc(a.part_ml + unit * 2),
+                                          local * 8, 0, kSc1);
+  }
+}
+
+// One wave joins the splits of U columns from `col` on (those past the tile's last are
+// left out), reading up to B loads of each at once: lane s holds split s's (max, sum);
+// the weighted rows then run over 16 bytes per lane, HD / 4 lanes a row.
+template <int HD, int U, int B>
+__device__ __forceinline__ void join_columns(const PagedAttnArgs& a, const Item& t, int cols, int col, int hop, const float* ml0,
+                                             const float* src) {
+  constexpr int LPR = HD / 4, SPL = LLMRS_WAVE / LPR;
+  const int lane = lane_id(), ns = t.n_split, end = min(t.n_col - t.tile * cols, cols);
+  float w[U];
+  f32x4 acc[U];
+  dev_u32x2 ml[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(dev_rsrc(ml0), (min(lane, ns - 1) * hop + min(col + u, end - 1)) * 8, 0, kSc1);
+  }
+  for (int s0 = 0; s0 < ns; s0 += SPL * B) {
+    dev_u32x4 x[U][B];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < B; ++k)
+        x[u][k] = __builtin_amdgcn_raw_buffer_load_b128(
+            dev_rsrc(src),
+            ((min(s0 + k * SPL + lane / LPR, ns - 1) * hop + min(col + u, end - 1)) * HD + 4 * (lane % LPR)) * 4, 0, kSc1);
+    if (s0 == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float ms = lane < ns ? __uint_as_float(ml[u].x) : kNone;
+        w[u] = __builtin_amdgcn_exp2f(ms - wave_max(ms)) * (lane < ns ? __uint_as_float(ml[u].y) : 0.0f);
+        w[u] = w[u] / wave_sum(w[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < B; ++k) {  // splits past the last: weight 0 (their lanes hold none)
+        const int s = s0 + k * SPL + lane / LPR;
+        const float f = __shfl(w[u], s & 63);
+        acc[u] = acc[u] + __builtin_bit_cast(f32x4, x[u][k]) * (s < ns ? f : 0.0f);
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (SPL == 4) acc[u][i] += xor16(acc[u][i]);
+      acc[u][i] += xor32(acc[u][i]);
+    }
+    if (lane < LPR && col + u < end) *(f32x4*)(out_row(a, t, t.tile * cols + col + u, HD) + 4 * lane) = acc[u];
   }
 }
 
 // The tile's last workgroup (a ticket, no waiting) joins the splits, in split
 // order: what it reads moved with device-scope stores, each waited for before the
-// ticket was taken.  A wave takes a column: lane s holds split s's (max, sum); the
-// weighted rows then run over 16 bytes per lane, HD / 4 lanes a row.
+// ticket was taken.  (Through one XCD's L2 instead, where a head's workgroups share
+// one: 22.1 -> 21.7 us over 8 x 32768 positions, 30.4 -> 31.6 with 40 columns; not kept.)
+// Its time is that of its rounds of loads, so a wave takes four columns at a time
+// where a few splits leave it the registers, and else two.
 template <int HD>
 __device__ __forceinline__ void join_splits(const PagedAttnArgs& a, const Item& t, int cols, int* ticket) {
   if (t.n_split == 1) return;
-  const int nkv = a.pool.nkv, lane = lane_id();
+  const int nkv = a.pool.nkv;
   const size_t first = (size_t)(t.item - t.split) * nkv + t.head;
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  if (threadIdx.x == 0) *ticket = atomicAdd(a.tickets + first * kTicketStride, 1);
+  int* counter = a.tickets + first * kTicketStride;
+  if (threadIdx.x == 0) *ticket = atomicAdd(counter, 1);
   __syncthreads();
   if (*ticket != t.n_split - 1) return;
-  if (threadIdx.x == 0) dev_stu(a.tickets + first * kTicketStride, 0, 0u);  // as it was found, for the next launch
-  constexpr int LPR = HD / 4, SPL = LLMRS_WAVE / LPR, BATCH = 16;
+  if (threadIdx.x == 0) dev_stu(counter, 0, 0u);  // as it was found, for the next launch
   const float* ml0 = a.part_ml + first * cols * 2;
   const float* src = a.part_o + first * cols * HD;
-  const int hop = nkv * cols, tile_cols = min(t.n_col - t.tile * cols, cols), ns = t.n_split;
-  for (int col = __builtin_amdgcn_readfirstlane(wave_id()); col < tile_cols; col += kThreads / LLMRS_WAVE) {
-    const dev_u32x2 ml = dev_ld8(ml0, (min(lane, ns - 1) * hop + col) * 8);
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float w = 0.0f;
-    for (int s0 = 0; s0 < ns; s0 += SPL * BATCH) {
-      dev_u32x4 x[BATCH];
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k)
-        if (s0 + k * SPL < ns) x[k] = dev_ld16(src, ((min(s0 + k * SPL + lane / LPR, ns - 1) * hop + col) * HD + 4 * (lane % LPR)) * 4);
-      if (s0 == 0) {
-        const float ms = lane < ns ? __uint_as_float(ml.x) : -INFINITY;
-        const float M = wave_max(ms);
-        w = __builtin_amdgcn_exp2f(ms - (M == -INFINITY ? 0.0f : M)) * (lane < ns ? __uint_as_float(ml.y) : 0.0f);
-        w = w / wave_sum(w);
-      }
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k)
-        if (s0 + k * SPL < ns) acc = acc + __builtin_bit_cast(f32x4, x[k]) * __shfl(w, min(s0 + k * SPL + lane / LPR, 63));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (SPL == 4) acc[i] += xor16(acc[i]);
-      acc[i] += xor32(acc[i]);
-    }
-    if (lane < LPR) *(f32x4*)(out_row(a, t, t.tile * cols + col, HD) + 4 * lane) = acc;
+  const int end = min(t.n_col - t.tile * cols, cols), wave = __builtin_amdgcn_readfirstlane(wave_id());
+  constexpr int SPL = 256 / HD;  // splits of a load
+  if (t.n_split <= 2 * SPL) {
+    for (int col = 4 * wave; col < end; col += 16) join_columns<HD, 4, 2>(a, t, cols, col, nkv * cols, ml0, src);
+  } else {
+    for (int col = 2 * wave; col < end; col += 8) join_columns<HD, 2, 8>(a, t, cols, col, nkv * cols, ml0, src);
   }
 }
 
-// Up to 16 columns: the four waves take every fourth tile of the split each, with
+// 16 columns: the four waves take every fourth tile of the split each, with
 // the codes straight from the cache, and merge through LDS.  q is prepared by all
 // of them together, 16 lanes a column, while the first tile is on its way.
 template <int HD>
 __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
   constexpr int S = HD / 64, ND = HD / 16, MID = HD / 2, BYTES = kBlk * HD, WP = 4, COLS = 16, STEP = 64 * WP;
-  __shared__ __align__(16) float so[WP * COLS * HD];
+  __shared__ __align__(16) float so[WP * 16 * HD];
   __shared__ float sm[WP * COLS * 2];
   __shared__ __align__(16) i32x4 sq[3 * S * LLMRS_WAVE];
   __shared__ float ssl[COLS];
@@ -535,7 +615,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
     const int at = ((j >> 2) * 16 + (tid >> 4)) * 16;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      uint8_t* dst = (uint8_t*)sq + k * S * 1024 + at;
+      uint8_t* dst = (uint8_t*)(sq + k * S * LLMRS_WAVE) + at;
       if constexpr (HD == 128) {
         *(unsigned*)(dst + 4 * (j & 3)) = wu[k];
         *(unsigned*)(dst + 1024 + 4 * (j & 3)) = wv[k];
@@ -546,23 +626,26 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
     }
     if (j == 0) ssl[tid >> 4] = row_scale(a.scale, ex, odd);
   }
-  __syncthreads();
+  // a barrier for LDS alone: __syncthreads would wait for the tile as well
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   const float sl2 = ssl[c];
-  const int limit = t.past + min(col0 + c, t.n_col - 1) / t.n_rep, lowest = t.past + col0 / t.n_rep;
+  const int limit = t.past + min(col0 + c, t.n_col - 1) / t.n_rep;  // the column's last visible position
+  const int lowest = t.past + col0 / t.n_rep;
   Column<HD> x;
   for (; t0 < t.to; t0 += STEP) {
     const int ek = (int8_t)(exps & 255);
     const float ev = (float)(int8_t)(exps >> 8);
     float sv[16];
     asm volatile("" ::: "memory");  // q is read again for every tile: its registers are worth more
-    const float mx = Column<HD>::scores([&](int b, int s) { return kk[b][s]; },
-                                        [&](int k, int s) { return sq[(k * S + s) * LLMRS_WAVE + lane]; }, t0 + 63 > lowest,
-                                        limit - t0 - 16 * r, sv);
+    Column<HD>::template scores<4>([&](int b, int s) { return kk[b][s]; },
+                                    [&](int k, int s) { return sq[(k * S + s) * LLMRS_WAVE + lane]; }, sv);
+    if (t0 + 63 > lowest) Column<HD>::hide(limit - t0 - 16 * r, sv);
     __builtin_amdgcn_sched_barrier(0);
     if (t0 + STEP < t.to) fetch_k(t0 + STEP);
     __builtin_amdgcn_sched_barrier(0);
     h16x8 ph[2], pl[2];
-    x.weigh(sv, mx, sl2, ek, ev, ph, pl);
+    x.weigh(sv, sl2, ek, ev, ph, pl);
+    x.rescale();
     // two dim blocks at a time: their products are independent of each other
 #pragma unroll
     for (int d0 = 0; d0 < ND; d0 += 2) {
@@ -574,32 +657,34 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int d = 0; d < 2; ++d) x.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d][h], ph[h], x.o[d0 + d], 0, 0, 0);
+        for (int d = 0; d < 2; ++d)
+          x.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d][h], ph[h], x.o[d0 + d], 0, 0, 0);
 #pragma unroll
-        for (int d = 0; d < 2; ++d) x.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d][h], pl[h], x.o[d0 + d], 0, 0, 0);
+        for (int d = 0; d < 2; ++d)
+          x.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d][h], pl[h], x.o[d0 + d], 0, 0, 0);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     if (t0 + STEP < t.to) fetch_v();
     __builtin_amdgcn_sched_barrier(0);
   }
+  // the waves' results, in order; wave 0 has the sum
   x.close();
 #pragma unroll
-  for (int d = 0; d < ND; ++d) *(f32x4*)(so + (wave * COLS + c) * HD + 16 * d + 4 * r) = x.o[d];
+  for (int d = 0; d < ND; ++d) *(f32x4*)(so + (wave * 16 + c) * HD + 16 * d + 4 * r) = x.o[d];
   if (r == 0) {
-    sm[(wave * COLS + c) * 2] = x.m;
-    sm[(wave * COLS + c) * 2 + 1] = x.l;
+    sm[(wave * 16 + c) * 2] = x.m;
+    sm[(wave * 16 + c) * 2 + 1] = x.l;
   }
   __syncthreads();
   if (wave == 0) {
     float M = x.m;
 #pragma unroll
-    for (int w = 1; w < WP; ++w) M = fmaxf(M, sm[(w * COLS + c) * 2]);
-    const float at = M == -INFINITY ? 0.0f : M;
+    for (int w = 1; w < WP; ++w) M = fmaxf(M, sm[(w * 16 + c) * 2]);
     float L = 0.0f, cw[WP];
 #pragma unroll
     for (int w = 0; w < WP; ++w) {
-      cw[w] = __builtin_amdgcn_exp2f(sm[(w * COLS + c) * 2] - at) * sm[(w * COLS + c) * 2 + 1];
+      cw[w] = __builtin_amdgcn_exp2f(sm[(w * 16 + c) * 2] - M) * sm[(w * 16 + c) * 2 + 1];
       L += cw[w];
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -607,7 +692,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
     for (int d = 0; d < ND; ++d) {
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < WP; ++w) acc = acc + *(const f32x4*)(so + (w * COLS + c) * HD + 16 * d + 4 * r) * (cw[w] * inv);
+      for (int w = 0; w < WP; ++w) acc = acc + *(const f32x4*)(so + (w * 16 + c) * HD + 16 * d + 4 * r) * (cw[w] * inv);
       x.o[d] = acc;
     }
     x.m = M;
@@ -617,59 +702,69 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
   join_splits<HD>(a, t, COLS, &ticket);
 }
 
-// More columns: a wave has 16 NG of its own and takes every tile of the split.  The
+// More columns: each wave has 16 of its own and takes every tile of the split.  The
 // workgroup brings a tile into LDS once, V already as f16, while the one before is
 // computed.
-template <int HD, int NG>
+template <int HD>
 __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
-  constexpr int S = HD / 64, ND = HD / 16, MID = HD / 2, BYTES = kBlk * HD, COLS = 64 * NG;
+  constexpr int S = HD / 64, ND = HD / 16, MID = HD / 2, BYTES = kBlk * HD, COLS = 64, T = kThreads;
   constexpr int KW = 4 * S * LLMRS_WAVE, VW = 2 * ND * LLMRS_WAVE;  // 16-byte words of a tile
   constexpr int PER = BYTES / 16;                                   // of a block's K or V codes
-  constexpr int N = 2 * PER / kThreads;                             // of them per thread and tile: 1 or 2
+  constexpr int N = (2 * PER + T - 1) / T;                          // of them per thread and tile
+  constexpr int DB = 2;                                             // dim blocks at a time
   __shared__ __align__(16) u32x4 sk[2][KW];
   __shared__ __align__(16) u32x4 sv16[2][VW];
   __shared__ int ticket;
   const Item t = item_of(a, COLS);
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int c = lane & 15, r = lane >> 4;
-  const int col0 = t.tile * COLS + wave * 16 * NG;
+  const int col0 = t.tile * COLS + wave * 16;
 
-  // word w of block j of the tile
+  // word w of a tile: word w % PER of its block w / PER
   u32x4 gk[N], gv[N];
+  auto fetch = [&](u32x4 (&g)[N], const Place& p, int v) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int w = tid + n * T;
+      if (2 * PER % T == 0 || w < 2 * PER)
+        g[n] = ((const u32x4*)(a.pool.codes + ((w < PER ? p.u0 : p.u1) + v) * BYTES))[w % PER];
+    }
+  };
+  auto stage_k = [&](int buf) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int w = tid + n * T, j = w / PER, i = w % PER;
+      if (2 * PER % T == 0 || w < 2 * PER) sk[buf][(i >> 3) * 16 + j * 8 + (i & 7)] = gk[n];
+    }
+  };
+  auto stage_v = [&](int buf) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      // word (d, r2, c): positions 16 (2 j + r2) .. of dim 16 d + c
+      const int w = tid + n * T, j = w / PER, i = w % PER;
+      const int d = i >> 5, at = (2 * j + ((i >> 4) & 1)) * 16 + (i & 15);
+      if (2 * PER % T == 0 || w < 2 * PER)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          sv16[buf][(d * 2 + h) * LLMRS_WAVE + at] = __builtin_bit_cast(u32x4, v_half(gv[n][2 * h], gv[n][2 * h + 1]));
+    }
+  };
+  auto exps_of = [&](const Place& p) { return *(const uint16_t*)(a.pool.exps + (r < 2 ? p.u0 : p.u1)); };
+  const int n_tile = max(t.to - t.from + 63, 0) / 64;
   unsigned exps = 0, exps_next = 0;
-  auto fetch = [&](int t0) {
+  auto fetch_tile = [&](int t0) {
     const Place p = place_of(a, t, t0);
-    exps_next = *(const uint16_t*)(a.pool.exps + (r < 2 ? p.u0 : p.u1));
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int j = N == 2 ? n : tid / PER, w = N == 2 ? tid : tid % PER;
-      const u32x4* src = (const u32x4*)(a.pool.codes + (j ? p.u1 : p.u0) * BYTES) + w;
-      gk[n] = src[0];
-      gv[n] = src[PER];
-    }
+    exps_next = exps_of(p);
+    fetch(gk, p, 0);
+    fetch(gv, p, 1);
   };
-  auto stage = [&](int buf) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int j = N == 2 ? n : tid / PER, w = N == 2 ? tid : tid % PER;
-      sk[buf][(w >> 3) * 16 + j * 8 + (w & 7)] = gk[n];
-      // V word (d, r2, c): positions 16 (2 j + r2) .. of dim 16 d + c
-      const int d = w >> 5, at = (2 * j + ((w >> 4) & 1)) * 16 + (w & 15);
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        sv16[buf][(d * 2 + h) * LLMRS_WAVE + at] = __builtin_bit_cast(u32x4, v_half(gv[n][2 * h], gv[n][2 * h + 1]));
-    }
-  };
-  if (t.from < t.to) fetch(t.from);
+  if (n_tile) fetch_tile(t.from);
   __builtin_amdgcn_sched_barrier(0);
 
-  i32x4 qb[NG][3][S];
-  float sl2[NG];
-  int limit[NG];  // the column's last visible position
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const int col = min(col0 + 16 * g + c, t.n_col - 1);
-    limit[g] = t.past + col / t.n_rep;
+  i32x4 qb[3][S];
+  float sl2;
+  const int col = min(col0 + c, t.n_col - 1), limit = t.past + col / t.n_rep;  // the column's last visible position
+  {
     const float* x = a.q + ((size_t)(t.q.row0 + col / t.n_rep) * a.nq + t.head * t.n_rep + col % t.n_rep) * HD;
     float v[S][16];
 #pragma unroll
@@ -680,7 +775,7 @@ __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
         v[s][e] = w.x; v[s][e + 1] = w.y; v[s][e + 2] = w.z; v[s][e + 3] = w.w;
       }
     if (a.rope_cos) {
-      const size_t at = (size_t)limit[g] * MID + (HD == 128 ? 16 : 8) * r;
+      const size_t at = (size_t)limit * MID + (HD == 128 ? 16 : 8) * r;
 #pragma unroll
       for (int e = 0; e < (HD == 128 ? 16 : 8); ++e) {
         const float cs = a.rope_cos[at + e], sn = a.rope_sin[at + e];
@@ -713,71 +808,62 @@ __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) put_bytes(odd ? 0.0f : v[s][4 * k + b], ex, b, w);
 #pragma unroll
-        for (int n = 0; n < 3; ++n) qb[g][n][s][k] = (int)w[n];
+        for (int n = 0; n < 3; ++n) qb[n][s][k] = (int)w[n];
       }
-    sl2[g] = row_scale(a.scale, ex, odd);
+    sl2 = row_scale(a.scale, ex, odd);
   }
-  // the wave's own range: from a tile that all of its columns see to the last that
-  // one of them does
+  // the wave's own range: tiles that all of its columns see, and the last that one
+  // of them does
   const int lowest = t.past + min(col0, t.n_col - 1) / t.n_rep;
-  const int last = col0 < t.n_col ? t.past + (min(col0 + 16 * NG, t.n_col) - 1) / t.n_rep : -1;
-  Column<HD> x[NG];
+  const int last = col0 < t.n_col ? t.past + (min(col0 + 16, t.n_col) - 1) / t.n_rep : -1;
+  Column<HD> x;
   exps = exps_next;
-  if (t.from < t.to) stage(0);
+  if (n_tile) {
+    stage_k(0);
+    stage_v(0);
+  }
   __syncthreads();
-  int buf = 0;
-  for (int t0 = t.from; t0 < t.to; t0 += 64, buf ^= 1) {
-    const bool more = t0 + 64 < t.to;
-    if (more) fetch(t0 + 64);
+  for (int n = 0; n < n_tile; ++n) {
+    const int t0 = t.from + 64 * n, buf = n & 1;
+    fetch_tile(min(t0 + 64, t.from + 64 * (n_tile - 1)));  // after the last: that one again, not used
     __builtin_amdgcn_sched_barrier(0);
     if (t0 <= last) {
-      const int ek = (int8_t)(exps & 255);
-      const float ev = (float)(int8_t)(exps >> 8);
-      h16x8 ph[NG][2], pl[NG][2];
+      float sv[16];
+      Column<HD>::template scores<2>([&](int b, int s) { return __builtin_bit_cast(i32x4, sk[buf][(b * S + s) * LLMRS_WAVE + lane]); },
+                                      [&](int k, int s) { return qb[k][s]; }, sv);
+      if (t0 + 63 > lowest) Column<HD>::hide(limit - t0 - 16 * r, sv);
+      h16x8 ph[2], pl[2];
+      x.weigh(sv, sl2, (int8_t)(exps & 255), (float)(int8_t)(exps >> 8), ph, pl);
+      x.rescale();
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float sv[16];
-        const float mx = Column<HD>::scores(
-            [&](int b, int s) { return __builtin_bit_cast(i32x4, sk[buf][(b * S + s) * LLMRS_WAVE + lane]); },
-            [&](int k, int s) { return qb[g][k][s]; }, t0 + 63 > lowest, limit[g] - t0 - 16 * r, sv);
-        x[g].weigh(sv, mx, sl2[g], ek, ev, ph[g], pl[g]);
-      }
-#pragma unroll
-      for (int d0 = 0; d0 < ND; d0 += 2)
+      for (int d0 = 0; d0 < ND; d0 += DB)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          h16x8 va[2];
+          h16x8 va[DB];
 #pragma unroll
-          for (int d = 0; d < 2; ++d) va[d] = __builtin_bit_cast(h16x8, sv16[buf][((d0 + d) * 2 + h) * LLMRS_WAVE + lane]);
+          for (int d = 0; d < DB; ++d) va[d] = __builtin_bit_cast(h16x8, sv16[buf][((d0 + d) * 2 + h) * LLMRS_WAVE + lane]);
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
+          for (int d = 0; d < DB; ++d) x.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d], ph[h], x.o[d0 + d], 0, 0, 0);
 #pragma unroll
-            for (int d = 0; d < 2; ++d)
-              x[g].o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d], ph[g][h], x[g].o[d0 + d], 0, 0, 0);
-#pragma unroll
-            for (int d = 0; d < 2; ++d)
-              x[g].o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d], pl[g][h], x[g].o[d0 + d], 0, 0, 0);
-          }
+          for (int d = 0; d < DB; ++d) x.o[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d], pl[h], x.o[d0 + d], 0, 0, 0);
         }
     }
     exps = exps_next;
-    if (more) stage(buf ^ 1);
+    stage_k(buf ^ 1);
+    stage_v(buf ^ 1);
     __syncthreads();
   }
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    x[g].close();
-    put_column<HD>(a, t, COLS, wave * 16 * NG + 16 * g + c, x[g]);
-  }
+  x.close();
+  put_column<HD>(a, t, COLS, wave * 16 + c, x);
   join_splits<HD>(a, t, COLS, &ticket);
 }
 
-extern "C" __global__ __launch_bounds__(kThreads, 2) void paged_attn_hd64_few(PagedAttnArgs a) { attend_few<64>(a); }
-extern "C" __global__ __launch_bounds__(kThreads, 2) void paged_attn_hd128_few(PagedAttnArgs a) { attend_few<128>(a); }
-extern "C" __global__ __launch_bounds__(kThreads, 2) void paged_attn_hd64_many1(PagedAttnArgs a) { attend_many<64, 1>(a); }
-extern "C" __global__ __launch_bounds__(kThreads, 2) void paged_attn_hd128_many1(PagedAttnArgs a) { attend_many<128, 1>(a); }
-extern "C" __global__ __launch_bounds__(kThreads, 2) void paged_attn_hd64_many2(PagedAttnArgs a) { attend_many<64, 2>(a); }
-extern "C" __global__ __launch_bounds__(kThreads, 2) void paged_attn_hd128_many2(PagedAttnArgs a) { attend_many<128, 2>(a); }
+#define LLMRS_PAGED_ATTN(KIND, HD, WAVES, BODY)                                                               \
+  extern "C" __global__ __launch_bounds__(kThreads, WAVES) void paged_attn_##KIND##_hd##HD(PagedAttnArgs a) { BODY; }
+LLMRS_PAGED_ATTN(few, 64, 3, attend_few<64>(a))
+LLMRS_PAGED_ATTN(many, 64, 3, attend_many<64>(a))
+LLMRS_PAGED_ATTN(few, 128, 2, attend_few<128>(a))
+LLMRS_PAGED_ATTN(many, 128, 3, attend_many<128>(a))
 
 // Words of the host into device memory (words.h).
 extern "C" __global__ __launch_bounds__(kThreads) void paged_words(WordsArgs a) {

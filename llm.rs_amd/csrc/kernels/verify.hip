@@ -32,9 +32,12 @@ struct Row {
 // drawn from.  One draft per lane.
 __device__ __forceinline__ Row examine(const VerifyArgs& a, int i) {
   Row r;
-  const int row = word(a, 3 * i);
-  r.first = word(a, 3 * i + 1);
-  r.drafts = word(a, 3 * i + 2);
+  // (one value per wave: the compiler takes what is loaded from either of two places
+  // to differ from lane to lane)
+  auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int row = uni(word(a, 3 * i));
+  r.first = uni(word(a, 3 * i + 1));
+  r.drafts = uni(word(a, 3 * i + 2));
   const int lane = lane_id(), base = 3 * a.n + r.first;
   bool refused = false;
   if (lane < r.drafts) {
@@ -49,7 +52,7 @@ __device__ __forceinline__ Row examine(const VerifyArgs& a, int i) {
   r.p = a.target + (size_t)(row + r.accepted) * a.vocab;
   const bool rest = r.accepted < r.drafts;
   r.q = rest && a.draft ? a.draft + (size_t)(r.first + r.accepted) * a.vocab : nullptr;
-  r.drafted = rest && !a.draft ? word(a, base + r.accepted) : -1;
+  r.drafted = rest && !a.draft ? uni(word(a, base + r.accepted)) : -1;
   return r;
 }
 

@@ -95,7 +95,9 @@ class RefCache:
         delta bounds the relative error of an unnormalised weight: q rotated in
         f32 (3 roundings) and rounded to 22 bits below its row's largest value, the
         score's f32 sum, product and scale (8 roundings of its size), log2(e) and exp2
-        (4 roundings).  A sum of n weighted values in f32, in whatever order, adds n
+        (4 roundings).  The sum of the lowest of q's three bytes times the codes counts in
+        whole steps of 2^8: q's integer is at most 2^22, so a step is 2^8 / 2^21 = 2^-13 of
+        q's largest value (an integer in (2^21, 2^22]) times one step of K.  A sum of n weighted values in f32, in whatever order, adds n
         roundings of sum p |v|; the weights are split in 22 bits, and joining and dividing
         add a few.  A weight p * 2^e is held as f16 hi + lo with the largest at 2^14: where
         lo has f16's smallest step, 2^-24, it is off by up to half of that, 2^-25 / 2^14 =
@@ -105,7 +107,7 @@ class RefCache:
         out, tol, row = [], [], 0
         for s, n in zip(slots, counts):
             k, v = self.values(s)
-            length, exps = k.shape[0], self._slot(s)["exps"][1]
+            length, (kexps, exps) = k.shape[0], self._slot(s)["exps"]
             x = q[row:row + n].astype(np.float64).reshape(n, nq, self.hd)
             row += n
             if self.rope is not None:
@@ -120,7 +122,8 @@ class RefCache:
                     p /= p.sum()
                     o[i, h] = p @ vv
                     size = np.abs(kk) @ np.abs(x[i, h]) / math.sqrt(self.hd)
-                    fixed = np.abs(x[i, h]).max() * 2.0 ** -23 * np.abs(kk).sum(1) / math.sqrt(self.hd)
+                    kstep = np.ldexp(1.0, [kexps[j // BLOCK, h // rep] for j in range(seen)])
+                    fixed = np.abs(x[i, h]).max() * (2.0 ** -23 * np.abs(kk).sum(1) + 2.0 ** -13 * kstep) / math.sqrt(self.hd)
                     delta = float(np.max(6 * u * size + 8 * u * np.abs(sc) + 8 * u * np.abs(sc - sc.max()) + fixed)) + 8 * u
                     step = np.ldexp(1.0, [exps[j // BLOCK, h // rep] for j in range(seen)])
                     floor = 2.0 ** -39 * np.max(p * step) * (np.abs(vv) / step[:, None]).sum(0)
