@@ -158,7 +158,8 @@ void launch_rows(const llmrs_paged* p, const std::string& kernel, const std::vec
   a.seqs.n = (int)parts.size();
   const LaunchWords words(seq_words(parts, items, &a.seqs.items), a.seqs.w);
   a.seqs.ext = words.ext();
-  launch(kernel + hd_tag(p), dim3((unsigned)a.seqs.items, (unsigned)p->cfg.n_kv_heads, 2), dim3(256), 0, ctx().stream, a);
+  launch(kernel + hd_tag(p), dim3((unsigned)a.seqs.items, (unsigned)p->cfg.n_kv_heads, 2),
+         dim3((unsigned)(2 * p->cfg.head_dim)), 0, ctx().stream, a);
 }
 
 // A kernel's columns per workgroup and the positions that its waves take at a time.

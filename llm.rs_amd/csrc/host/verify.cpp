@@ -15,20 +15,20 @@ void require_rows(const llmrs_tensor* t, size_t rows, size_t vocab, const char* 
                 std::string("verify_drafts: ") + what + " must be [" + std::to_string(rows) + ", " + std::to_string(vocab) + "]");
 }
 
-// Waits until every row starts with its stamp.  The kernel stores it last, so the
-// host sees it about 5 us before hipStreamSynchronize returns (an empty kernel,
-// launch to return: 6.6 against 11.5 us); work that is not done within a millisecond is
-// waited for there.
-void wait_for_stamps(const int* rows, size_t n, size_t row, int stamp) {
+// Waits until every word bears the stamp.  The host sees them about 5 us before
+// hipStreamSynchronize returns (an empty kernel, launch to return: 6.6 against 11.5
+// us); work that is not done within a millisecond is waited for there.
+void wait_for_stamps(const uint64_t* words, size_t n) {
   const auto until = std::chrono::steady_clock::now() + std::chrono::milliseconds(1);
+  auto there = [&](size_t i) { return __atomic_load_n(words + i, __ATOMIC_ACQUIRE) >> 32 == kVerifyStamp; };
   for (size_t i = 0; i < n;) {
-    if (__atomic_load_n(rows + i * row, __ATOMIC_ACQUIRE) == stamp) ++i;
+    if (there(i)) ++i;
     else if (std::chrono::steady_clock::now() > until) break;
   }
   for (size_t i = 0; i < n; ++i)
-    if (__atomic_load_n(rows + i * row, __ATOMIC_ACQUIRE) != stamp) {
+    if (!there(i)) {
       LLMRS_HIP(hipStreamSynchronize(ctx().stream));
-      LLMRS_REQUIRE(__atomic_load_n(rows + i * row, __ATOMIC_ACQUIRE) == stamp, LLMRS_E_HIP, "verify_drafts: no answer");
+      LLMRS_REQUIRE(there(i), LLMRS_E_HIP, "verify_drafts: no answer");
     }
 }
 
@@ -85,7 +85,7 @@ extern "C" int llmrs_verify_drafts(const llmrs_tensor* target, const llmrs_tenso
     a.groups = verify_groups((int)vocab);
     a.most = (int)most;
     a.drafts = (int)total;
-    const size_t row = 3 + most, bytes = 4 * n * row;
+    const size_t row = 2 + most, bytes = 8 * n * row;
     // tickets: zeroed here, and by each sequence's last workgroup
     if (c.n_verify_tickets < n) {
       if (c.verify_tickets) c.alloc.release(c.verify_tickets);
@@ -100,30 +100,29 @@ extern "C" int llmrs_verify_drafts(const llmrs_tensor* target, const llmrs_tenso
     Scratch part(8 * n * (size_t)a.groups), out(direct ? 0 : bytes);
     a.part = (double*)part.p;
     a.tickets = (int*)c.verify_tickets;
-    a.out = direct ? (int*)c.host_out : (int*)out.p;
-    a.stamp = 1;
+    a.out = direct ? (unsigned long long*)c.host_out : (unsigned long long*)out.p;
     // slices per wave: as many as leave four workgroups per CU; each looks at all
     // of its sequence's drafts first
     const size_t groups4 = ((size_t)a.groups + 3) / 4;
     a.per_wave = (int)std::max<size_t>(1, n * groups4 / (4 * (size_t)c.num_cus));
     const unsigned grid = (unsigned)((groups4 + a.per_wave - 1) / a.per_wave);
     if (direct)
-      for (size_t i = 0; i < n; ++i) __atomic_store_n((int*)c.host_out + i * row, 0, __ATOMIC_RELAXED);
+      for (size_t i = 0; i < n * row; ++i) __atomic_store_n((uint64_t*)c.host_out + i, 0, __ATOMIC_RELAXED);
     LaunchWords words(w, a.w);
     a.ext = words.ext();
     launch("verify_rows", dim3(grid, (unsigned)n), dim3(256), 0, c.stream, a);
-    std::vector<int> big;
-    const int* got = (const int*)c.host_out;
+    std::vector<uint64_t> big;
+    const uint64_t* got = (const uint64_t*)c.host_out;
     if (direct) {
-      wait_for_stamps((const int*)c.host_out, n, row, a.stamp);
+      wait_for_stamps(got, n * row);
     } else {
       big.resize(n * row);
       fetch(big.data(), out.p, bytes);
       got = big.data();
     }
     for (size_t i = 0; i < n; ++i) {
-      accepted[i] = got[i * row + 1];
-      for (size_t j = 0; j < width; ++j) tokens[i * width + j] = j <= most ? got[i * row + 2 + j] : -1;
+      accepted[i] = (int32_t)got[i * row];
+      for (size_t j = 0; j < width; ++j) tokens[i * width + j] = j <= most ? (int32_t)got[i * row + 1 + j] : -1;
     }
   });
 }

@@ -529,15 +529,16 @@ struct PagedAttnArgs {
 constexpr int kVerifySlice = 512;  // ids of one sum (a wave's, 8 per lane)
 constexpr int kVerifyMaxDrafts = 64;
 constexpr int verify_groups(int vocab) { return (vocab + kVerifySlice - 1) / kVerifySlice; }
+constexpr unsigned kVerifyStamp = 1;  // upper half of a word that is there
 struct VerifyArgs {
   const float* target;   // [rows][vocab]
   const float* draft;    // [drafted rows][vocab] (null: probability 1 at the drafted id)
   double* part;          // [sequence][group] sums of a slice
   int* tickets;          // [sequence][kTicketStride], zero between launches
-  int* out;              // [sequence][3 + most]: stamp, accepted, its tokens (-1 past the last); the host's memory
+  // [sequence][2 + most]: accepted, its tokens (-1 past the last), each below a stamp; the host's memory
+  unsigned long long* out;
   int vocab, n, groups, most;
   int per_wave;          // slices of a wave
-  int stamp;             // what a finished row starts with
   // words (as PagedSeqs): per sequence its first target row, first drafted row and
   // drafts; then the drafted ids, their uniform numbers (f32 bits), the draws
   const int* ext;

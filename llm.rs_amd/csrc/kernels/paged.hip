@@ -79,131 +79,190 @@ __device__ __forceinline__ int shift_code(int c, int d) {
   return d ? (c + ((1 << (d - 1)) - 1) + ((c >> d) & 1)) >> d : c;
 }
 
-// Largest magnitude the format holds; NaN counts as zero.
-__device__ __forceinline__ double storable(double x) {
-  constexpr double top = 127.0 * 2658455991569831745807614120560689152.0;  // 127 * 2^121
-  return x != x ? 0.0 : fmin(fmax(x, -top), top);
+// Within the magnitudes that the format holds; NaN counts as zero.
+template <class T>
+__device__ __forceinline__ T storable(T x) {
+  constexpr T top = T(127.0 * 2658455991569831745807614120560689152.0);  // 127 * 2^121
+  return x != x ? T(0) : x < -top ? -top : x > top ? top : x;
 }
+
+// A word of four older codes, rounded to a step 2^d times theirs.
+__device__ __forceinline__ unsigned shift_word(unsigned w, int d, int bias) {
+  unsigned out = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    out |= ((unsigned)(shift_code((int)(int8_t)((w >> (8 * b)) ^ (unsigned)bias), d) + bias) & 255u) << (8 * b);
+  return out;
+}
+// Bytes [0, n) of the one, the others of the other (n may be any number).
+__device__ __forceinline__ unsigned first_bytes(unsigned w, unsigned other, int n) {
+  const unsigned mask = n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u;
+  return (w & mask) | (other & ~mask);
+}
+
+// Threads for a block of 32 positions of one KV head, K or V.
+constexpr int block_threads(int hd) { return 2 * hd; }
 
 }  // namespace
 
-// Appends rows to one block of one sequence.  The block's codes pass through LDS:
-// the older rows' are loaded and, where the new rows raise the exponent, rounded
-// to the new step.  K is rotated in 64 bits (the products of f32 values are exact
-// there), so a code does not depend on how a sum was rounded.
+// Appends rows to one block of one sequence.  A thread has 16 codes, and so nobody else
+// writes its bytes: of V a dim's 16 positions, of K four dims and their rotation
+// partners at two positions.  All its rows are asked for before the first is looked at.
+// Older codes are loaded and, where the new rows raise the exponent, rounded to the
+// new step.  K is rotated in 64 bits (the products of f32 values are exact there), so
+// a code does not depend on how a sum was rounded.
 template <int HD>
 __device__ __forceinline__ void append_block(const PagedRowsArgs& a) {
-  constexpr int MID = HD / 2, BYTES = kBlk * HD, ROWS = kBlk / (kThreads / MID);  // rows per thread
-  __shared__ __align__(16) uint8_t codes[BYTES];
-  __shared__ double red[kThreads / LLMRS_WAVE];
+  constexpr int MID = HD / 2, BYTES = kBlk * HD, LANES = MID / 4, WAVES = block_threads(HD) / LLMRS_WAVE;
+  __shared__ float red[WAVES];
   const int tid = threadIdx.x, head = blockIdx.y, which = blockIdx.z;
   const Seq q = find_seq(a.seqs, blockIdx.x);
   const int block = q.pos / kBlk + q.item;                  // of the sequence
   const int old = max(0, q.pos - block * kBlk);             // rows already there
   const int end = min(kBlk, q.pos + q.rows - block * kBlk); // rows after
-  const int pb = pool_block(a.pool, q.slot, block);
-  const size_t unit = ((size_t)pb * a.pool.nkv + head) * 2 + which;
+  const size_t unit = ((size_t)pool_block(a.pool, q.slot, block) * a.pool.nkv + head) * 2 + which;
   uint8_t* dst = a.pool.codes + unit * BYTES;
-
-  // this thread's values: rows old + g, old + g + G, ..., dims j and j + HD/2
-  constexpr int G = kThreads / MID;
-  const int j = tid % MID, g = tid / MID;
-  const int row0 = q.row0 + block * kBlk - q.pos, width = a.pool.nkv * HD;  // row of the block's position 0
-  const float* src = a.rows[which] + (size_t)head * HD + j;
-  const bool turn = which == 0 && a.rope_cos;
-  double lo[ROWS], hi[ROWS], amax = 0.0;
+  const int row0 = q.row0 + block * kBlk - q.pos;  // row of the block's position 0
+  // (a position without a new row: the nearest that has one)
+  auto near = [&](int p) { return min(max(p, old), end - 1); };
+  const float* src = a.rows[which] + (size_t)head * HD;
+  auto row = [&](int p) { return src + (size_t)(row0 + near(p)) * (a.pool.nkv * HD); };
+  auto exponent = [&](double amax) {  // of the block, from every thread's largest magnitude
+    float e = wave_max((float)needed_exp(amax));
+    if (lane_id() == 0) red[wave_id()] = e;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int p = i * G + g;
-    lo[i] = hi[i] = 0.0;
-    if (p >= old && p < end) {
-      const float* x = src + (size_t)(row0 + p) * width;
-      double u = x[0], w = x[MID];
-      if (turn) {
-        const size_t t = (size_t)(block * kBlk + p) * MID + j;
-        const double c = a.rope_cos[t], s = a.rope_sin[t], u0 = u;
-        u = u0 * c - w * s;
-        w = u0 * s + w * c;
-      }
-      lo[i] = storable(u);
-      hi[i] = storable(w);
-      amax = fmax(amax, fmax(fabs(lo[i]), fabs(hi[i])));
-    }
-  }
-  u32x4 was[BYTES / (16 * kThreads) ? BYTES / (16 * kThreads) : 1];
-  constexpr int VECS = BYTES / 16;
-  if (old)
-    for (int i = tid, n = 0; i < VECS; i += kThreads, ++n) was[n] = ((const u32x4*)dst)[i];
+    for (int w = 0; w < WAVES; ++w) e = fmaxf(e, red[w]);
+    return (int)e;
+  };
   const int e_old = old ? a.pool.exps[unit] : kPagedExpMin;
+  int e;
+  if (which) {
+    const int d = tid % HD, p0 = tid / HD * 16;
+    u32x4* at = (u32x4*)(dst + paged_v_offset(p0, d));
+    const bool adds = max(old, p0) < min(end, p0 + 16), has = old > p0;
+    float x[16], amax = 0.0f;
+    u32x4 was = {0, 0, 0, 0};
+    if (adds)
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) amax = fmax(amax, __shfl_xor(amax, o));
-  if (lane_id() == 0) red[wave_id()] = amax;
-  __syncthreads();
+      for (int i = 0; i < 16; ++i) x[i] = row(p0 + i)[d];
+    if (has) was = *at;
+    if (adds)
 #pragma unroll
-  for (int w = 0; w < kThreads / LLMRS_WAVE; ++w) amax = fmax(amax, red[w]);
-  const int e = max(e_old, needed_exp(amax));
-  const int bias = which ? 128 : 0;
-  if (old) {
-    const int d = min(e - e_old, 8);
-    for (int i = tid, n = 0; i < VECS; i += kThreads, ++n) {
-      u32x4 v = was[n];
-      if (d) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          unsigned out = 0;
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const int c = (int)(int8_t)((v[k] >> (8 * b)) ^ (which ? 0x80u : 0u));
-            out |= ((unsigned)(shift_code(c, d) + bias) & 255u) << (8 * b);
-          }
-          v[k] = out;
-        }
+      for (int i = 0; i < 16; ++i) {
+        x[i] = storable(x[i]);
+        amax = fmaxf(amax, fabsf(x[i]));
       }
-      ((u32x4*)codes)[i] = v;
-    }
-  }
-  __syncthreads();
+    e = max(e_old, exponent(amax));
+    if (has && e > e_old)
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int p = i * G + g;
-    if (p >= old && p < end) {
-      const int cl = (int)rint(ldexp(lo[i], -e)), ch = (int)rint(ldexp(hi[i], -e));
-      codes[which ? paged_v_offset(p, j) : paged_k_offset(p, j, HD)] = (uint8_t)(cl + bias);
-      codes[which ? paged_v_offset(p, j + MID) : paged_k_offset(p, j + MID, HD)] = (uint8_t)(ch + bias);
+      for (int k = 0; k < 4; ++k) was[k] = shift_word(was[k], min(e - e_old, 8), 128);
+    if (adds)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        unsigned w = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) w |= (unsigned)((int)rintf(ldexpf(x[4 * k + b], -e)) + 128) << (8 * b);
+        was[k] = first_bytes(was[k], w, old - p0 - 4 * k);
+      }
+    if (adds || has) *at = was;
+  } else {
+    const int d = 4 * (tid % LANES), p0 = tid / LANES;
+    const bool turn = a.rope_cos;
+    f32x4 x[2][2], cs[2], sn[2];
+    unsigned was[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = p0 + 16 * i;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[i][h] = *(const f32x4*)(row(p) + d + h * MID);
+      if (turn) {
+        const size_t t = (size_t)(block * kBlk + near(p)) * MID + d;
+        cs[i] = *(const f32x4*)(a.rope_cos + t);
+        sn[i] = *(const f32x4*)(a.rope_sin + t);
+      }
+      if (old)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) was[i][h] = *(const unsigned*)(dst + paged_k_offset(p, d + h * MID, HD));
+    }
+    double y[2][2][4], amax = 0.0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        double u = x[i][0][k], w = x[i][1][k];
+        if (turn) {
+          const double c = cs[i][k], s = sn[i][k], u0 = u;
+          u = u0 * c - w * s;
+          w = u0 * s + w * c;
+        }
+        y[i][0][k] = storable(u);
+        y[i][1][k] = storable(w);
+        amax = fmax(amax, fmax(fabs(y[i][0][k]), fabs(y[i][1][k])));
+      }
+    e = max(e_old, exponent(amax));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = p0 + 16 * i;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        unsigned w = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w |= ((unsigned)(int)rint(ldexp(y[i][h][k], -e)) & 255u) << (8 * k);
+        if (p < old) w = e > e_old ? shift_word(was[i][h], min(e - e_old, 8), 0) : was[i][h];
+        if (p < end) *(unsigned*)(dst + paged_k_offset(p, d + h * MID, HD)) = w;
+      }
     }
   }
-  __syncthreads();
-  for (int i = tid; i < VECS; i += kThreads) ((u32x4*)dst)[i] = ((const u32x4*)codes)[i];
   if (tid == 0) a.pool.exps[unit] = (int8_t)e;
 }
-extern "C" __global__ __launch_bounds__(kThreads) void paged_append_hd64(PagedRowsArgs a) { append_block<64>(a); }
-extern "C" __global__ __launch_bounds__(kThreads) void paged_append_hd128(PagedRowsArgs a) { append_block<128>(a); }
+extern "C" __global__ __launch_bounds__(block_threads(64)) void paged_append_hd64(PagedRowsArgs a) { append_block<64>(a); }
+extern "C" __global__ __launch_bounds__(block_threads(128)) void paged_append_hd128(PagedRowsArgs a) { append_block<128>(a); }
 
-// Reads one block's rows of a range back as f32.
+// Reads one block's rows of a range back as f32; a thread has the codes of the append.
 template <int HD>
 __device__ __forceinline__ void read_block(const PagedRowsArgs& a) {
-  constexpr int BYTES = kBlk * HD;
-  __shared__ __align__(16) uint8_t codes[BYTES];
+  constexpr int MID = HD / 2, BYTES = kBlk * HD, LANES = MID / 4;
   const int tid = threadIdx.x, head = blockIdx.y, which = blockIdx.z;
   const Seq q = find_seq(a.seqs, blockIdx.x);
   const int block = q.pos / kBlk + q.item;
   const int first = max(0, q.pos - block * kBlk), end = min(kBlk, q.pos + q.rows - block * kBlk);
   const size_t unit = ((size_t)pool_block(a.pool, q.slot, block) * a.pool.nkv + head) * 2 + which;
-  const u32x4* src = (const u32x4*)(a.pool.codes + unit * BYTES);
-  for (int i = tid; i < BYTES / 16; i += kThreads) ((u32x4*)codes)[i] = src[i];
+  const uint8_t* src = a.pool.codes + unit * BYTES;
   const float step = ldexpf(1.0f, a.pool.exps[unit]);
-  __syncthreads();
-  const int row0 = q.row0 + block * kBlk - q.pos, width = a.pool.nkv * HD;
   float* dst = a.rows[which] + (size_t)head * HD;
-  for (int i = tid; i < BYTES; i += kThreads) {
-    const int p = i / HD, d = i % HD;
-    if (p < first || p >= end) continue;
-    const int c = which ? (int)codes[paged_v_offset(p, d)] - 128 : (int)(int8_t)codes[paged_k_offset(p, d, HD)];
-    dst[(size_t)(row0 + p) * width + d] = (float)c * step;
+  auto row = [&](int p) { return dst + (ptrdiff_t)(q.row0 + block * kBlk - q.pos + p) * (a.pool.nkv * HD); };
+  if (which) {
+    const int d = tid % HD, p0 = tid / HD * 16;
+    if (max(first, p0) >= min(end, p0 + 16)) return;
+    const u32x4 w = *(const u32x4*)(src + paged_v_offset(p0, d));
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (p0 + i >= first && p0 + i < end)
+        row(p0 + i)[d] = (float)((int)((w[i / 4] >> (8 * (i % 4))) & 255u) - 128) * step;
+  } else {
+    const int d = 4 * (tid % LANES), p0 = tid / LANES;
+    unsigned w[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w[i][h] = *(const unsigned*)(src + paged_k_offset(p0 + 16 * i, d + h * MID, HD));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = p0 + 16 * i;
+      if (p < first || p >= end) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x4 x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = (float)((int)(w[i][h] << (24 - 8 * k)) >> 24) * step;
+        *(f32x4*)(row(p) + d + h * MID) = x;
+      }
+    }
   }
 }
-extern "C" __global__ __launch_bounds__(kThreads) void paged_read_hd64(PagedRowsArgs a) { read_block<64>(a); }
-extern "C" __global__ __launch_bounds__(kThreads) void paged_read_hd128(PagedRowsArgs a) { read_block<128>(a); }
+extern "C" __global__ __launch_bounds__(block_threads(64)) void paged_read_hd64(PagedRowsArgs a) { read_block<64>(a); }
+extern "C" __global__ __launch_bounds__(block_threads(128)) void paged_read_hd128(PagedRowsArgs a) { read_block<128>(a); }
 
 // Attention of new rows over the cached positions.  A column is one (row, query
 // head of the KV head's group); a wave takes 16 of them per group, and tiles of 64

@@ -159,7 +159,8 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const uns
       x[c] = g < groups ? __builtin_bit_cast(double, dev_ld8(part, 8 * g)) : 0.0;
     }
 #pragma unroll
-    for (int c = 0; c < kHeld; ++c) x[c] = scan(x[c]);
+    for (int c = 0; c < kHeld; ++c)
+      if (g0 + LLMRS_WAVE * c < groups) x[c] = scan(x[c]);
   };
   constexpr int HELD = LLMRS_WAVE * kHeld;
   double total = 0.0;
@@ -194,6 +195,7 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const uns
     if (groups > HELD) hold(g0);
 #pragma unroll
     for (int c = 0; c < kHeld; ++c) {
+      if (g0 + LLMRS_WAVE * c >= groups) break;
       const unsigned long long over = __ballot(base + x[c] > tau);
       const double before = dpp64<0x138, 0xF>(x[c]);
       const unsigned long long holds = __ballot(x[c] > before);
@@ -217,8 +219,7 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const uns
 // A wave sums slices of a sequence's row.  The sequence's last workgroup (a ticket, no
 // waiting; the sums move with device-scope stores and loads) draws, one wave of it
 // alone: the slice in which the running sum crosses, and the id in that slice.  Its
-// answer goes straight to the host's memory, where the caller waits for the stamp that
-// follows it.
+// answer goes straight to the host's memory, where the caller waits for the stamps.
 extern "C" __global__ __launch_bounds__(kThreads) void verify_rows(VerifyArgs a) {
   const int i = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(wave_id());
   const Row r = examine(a, i);
@@ -237,13 +238,11 @@ extern "C" __global__ __launch_bounds__(kThreads) void verify_rows(VerifyArgs a)
   if (__builtin_amdgcn_readfirstlane(ticket) != (int)gridDim.x - 1) return;
   if (tid == 0) dev_stu(a.tickets + (size_t)i * kTicketStride, 0, 0u);  // as it was found, for the next launch
   const int drawn = draw(a, r, part, __int_as_float(word(a, 3 * a.n + 2 * a.drafts + i)));
-  // words to the host's memory, each written through; the stamp once they are there
-  int* out = a.out + (size_t)i * (a.most + 3);
-  auto put = [](int* at, int v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); };
-  if (tid == 0) put(out + 1, r.accepted);
-  for (int j = tid; j <= a.most; j += LLMRS_WAVE)
-    put(out + 2 + j, j < r.accepted ? word(a, 3 * a.n + r.first + j) : j == r.accepted ? drawn : -1);
-  __builtin_amdgcn_s_waitcnt(0);
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  if (tid == 0) put(out, a.stamp);
+  // to the host's memory, each word with its stamp, so nothing waits for another
+  unsigned long long* out = a.out + (size_t)i * (a.most + 2);
+  for (int j = tid; j < a.most + 2; j += LLMRS_WAVE) {
+    const int at = j - 1;  // accepted drafts, tokens
+    const int v = j == 0 ? r.accepted : at < r.accepted ? word(a, 3 * a.n + r.first + at) : at == r.accepted ? drawn : -1;
+    __hip_atomic_store(out + j, (unsigned long long)kVerifyStamp << 32 | (unsigned)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
 }
