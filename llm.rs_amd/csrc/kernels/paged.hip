@@ -70,6 +70,7 @@ __device__ __forceinline__ int pool_block(const PagedPool& p, int slot, int b) {
 // The smallest e in [kPagedExpMin, kPagedExpMax] with amax <= 127 * 2^e: amax =
 // f * 2^x with f in [1/2, 1), and 127 = 127/128 * 2^7.
 __device__ __forceinline__ int needed_exp(double amax) {
+  amax = fmin(amax, 340282366920938463463374607431768211456.0);  // 2^128: infinities
   const int e = __builtin_amdgcn_frexp_exp(amax) - 7 + (__builtin_amdgcn_frexp_mant(amax) > 127.0 / 128.0 ? 1 : 0);
   return amax > 0.0 ? min(max(e, kPagedExpMin), kPagedExpMax) : kPagedExpMin;
 }
@@ -79,11 +80,18 @@ __device__ __forceinline__ int shift_code(int c, int d) {
   return d ? (c + ((1 << (d - 1)) - 1) + ((c >> d) & 1)) >> d : c;
 }
 
-// Within the magnitudes that the format holds; NaN counts as zero.
-template <class T>
-__device__ __forceinline__ T storable(T x) {
-  constexpr T top = T(127.0 * 2658455991569831745807614120560689152.0);  // 127 * 2^121
-  return x != x ? T(0) : x < -top ? -top : x > top ? top : x;
+// The code of a value: the nearest integer, half to even.  The conversions of the
+// hardware take NaN to 0 and what is too large to the ends of the range, which C++
+// leaves open.
+__device__ __forceinline__ int code_of(float x, int e) {
+  int c;
+  asm("v_cvt_i32_f32 %0, %1" : "=v"(c) : "v"(rintf(ldexpf(x, -e))));
+  return min(max(c, -127), 127);
+}
+__device__ __forceinline__ int code_of(double x, int e) {
+  int c;
+  asm("v_cvt_i32_f64 %0, %1" : "=v"(c) : "v"(rint(ldexp(x, -e))));
+  return min(max(c, -127), 127);
 }
 
 // A word of four older codes, rounded to a step 2^d times theirs.
@@ -138,21 +146,17 @@ __device__ __forceinline__ void append_block(const PagedRowsArgs& a) {
   const int e_old = old ? a.pool.exps[unit] : kPagedExpMin;
   int e;
   if (which) {
-    const int d = tid % HD, p0 = tid / HD * 16;
+    const int d = tid % HD, p0 = __builtin_amdgcn_readfirstlane(tid / HD * 16);
     u32x4* at = (u32x4*)(dst + paged_v_offset(p0, d));
     const bool adds = max(old, p0) < min(end, p0 + 16), has = old > p0;
-    float x[16], amax = 0.0f;
+    float x[16] = {}, amax = 0.0f;
     u32x4 was = {0, 0, 0, 0};
-    if (adds)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = row(p0 + i)[d];
     if (has) was = *at;
-    if (adds)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        x[i] = storable(x[i]);
-        amax = fmaxf(amax, fabsf(x[i]));
-      }
+    for (int i = 0; i < 16; ++i)
+      if (p0 + i >= old && p0 + i < end) x[i] = row(p0 + i)[d];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));  // passes over NaN
     e = max(e_old, exponent(amax));
     if (has && e > e_old)
 #pragma unroll
@@ -162,18 +166,26 @@ __device__ __forceinline__ void append_block(const PagedRowsArgs& a) {
       for (int k = 0; k < 4; ++k) {
         unsigned w = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) w |= (unsigned)((int)rintf(ldexpf(x[4 * k + b], -e)) + 128) << (8 * b);
+        for (int b = 0; b < 4; ++b) w |= (unsigned)(code_of(x[4 * k + b], e) + 128) << (8 * b);
         was[k] = first_bytes(was[k], w, old - p0 - 4 * k);
       }
     if (adds || has) *at = was;
   } else {
-    const int d = 4 * (tid % LANES), p0 = tid / LANES;
+    constexpr int ROWS = LLMRS_WAVE / LANES;  // of a wave, twice
+    const int d = 4 * (tid % LANES), p0 = tid / LANES, first = __builtin_amdgcn_readfirstlane(p0);
     const bool turn = a.rope_cos;
     f32x4 x[2][2], cs[2], sn[2];
     unsigned was[2][2];
+    bool adds[2], has[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int p = p0 + 16 * i;
+      const int p = p0 + 16 * i, from = first + 16 * i;
+      adds[i] = max(old, from) < min(end, from + ROWS);
+      has[i] = old > from;
+      if (has[i])
+#pragma unroll
+        for (int h = 0; h < 2; ++h) was[i][h] = *(const unsigned*)(dst + paged_k_offset(p, d + h * MID, HD));
+      if (!adds[i]) continue;
 #pragma unroll
       for (int h = 0; h < 2; ++h) x[i][h] = *(const f32x4*)(row(p) + d + h * MID);
       if (turn) {
@@ -181,13 +193,11 @@ __device__ __forceinline__ void append_block(const PagedRowsArgs& a) {
         cs[i] = *(const f32x4*)(a.rope_cos + t);
         sn[i] = *(const f32x4*)(a.rope_sin + t);
       }
-      if (old)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) was[i][h] = *(const unsigned*)(dst + paged_k_offset(p, d + h * MID, HD));
     }
     double y[2][2][4], amax = 0.0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+      if (!adds[i]) continue;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         double u = x[i][0][k], w = x[i][1][k];
@@ -196,19 +206,22 @@ __device__ __forceinline__ void append_block(const PagedRowsArgs& a) {
           u = u0 * c - w * s;
           w = u0 * s + w * c;
         }
-        y[i][0][k] = storable(u);
-        y[i][1][k] = storable(w);
-        amax = fmax(amax, fmax(fabs(y[i][0][k]), fabs(y[i][1][k])));
+        y[i][0][k] = u;
+        y[i][1][k] = w;
+        amax = fmax(amax, fmax(fabs(u), fabs(w)));  // passes over NaN
       }
+    }
     e = max(e_old, exponent(amax));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int p = p0 + 16 * i;
+      if (!adds[i] && !(has[i] && e > e_old)) continue;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         unsigned w = 0;
+        if (adds[i])
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w |= ((unsigned)(int)rint(ldexp(y[i][h][k], -e)) & 255u) << (8 * k);
+          for (int k = 0; k < 4; ++k) w |= ((unsigned)code_of(y[i][h][k], e) & 255u) << (8 * k);
         if (p < old) w = e > e_old ? shift_word(was[i][h], min(e - e_old, 8), 0) : was[i][h];
         if (p < end) *(unsigned*)(dst + paged_k_offset(p, d + h * MID, HD)) = w;
       }
