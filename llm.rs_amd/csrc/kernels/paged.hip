@@ -468,7 +468,7 @@ struct Item {
   Seq q;
   int item, head, n_rep, n_col, past, n_split, tile, split, from, to;
 };
-__device__ __forceinline__ Item item_of(const PagedAttnArgs& a, int cols) {
+__device__ __forceinline__ Item item_of(const PagedAttnArgs& a, int cols, int unit) {
   Item t;
   const int nkv = a.pool.nkv;
   t.head = blockIdx.x % nkv;
@@ -482,8 +482,9 @@ __device__ __forceinline__ Item item_of(const PagedAttnArgs& a, int cols) {
   t.split = t.q.item % t.n_split;
   t.tile = (t.n_col + cols - 1) / cols - 1 - t.tile;  // the last rows see the most: they come first
   // up to the last position that any of the tile's columns sees
-  t.from = t.split * a.chunk;
-  t.to = min(t.from + a.chunk, t.past + (min((t.tile + 1) * cols, t.n_col) - 1) / t.n_rep + 1);
+  const int chunk = ((t.q.pos + unit - 1) / unit + t.n_split - 1) / t.n_split * unit;  // splits of one length
+  t.from = t.split * chunk;
+  t.to = min(t.from + chunk, t.past + (min((t.tile + 1) * cols, t.n_col) - 1) / t.n_rep + 1);
   return t;
 }
 __device__ __forceinline__ float* out_row(const PagedAttnArgs& a, const Item& t, int col, int hd) {
@@ -615,7 +616,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
   __shared__ __align__(16) i32x4 sq[3 * S * LLMRS_WAVE];
   __shared__ float ssl[COLS];
   __shared__ int ticket;
-  const Item t = item_of(a, COLS);
+  const Item t = item_of(a, COLS, STEP);
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int c = lane & 15, r = lane >> 4;
   const int col0 = t.tile * COLS;
@@ -787,7 +788,7 @@ __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
   __shared__ __align__(16) u32x4 sk[2][KW];
   __shared__ __align__(16) u32x4 sv16[2][VW];
   __shared__ int ticket;
-  const Item t = item_of(a, COLS);
+  const Item t = item_of(a, COLS, 64);
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int c = lane & 15, r = lane >> 4;
   const int col0 = t.tile * COLS + wave * 16;
