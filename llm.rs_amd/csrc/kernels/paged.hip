@@ -290,12 +290,12 @@ extern "C" __global__ __launch_bounds__(block_threads(128)) void paged_read_hd12
 //   O^T += V^T P^T v_mfma_f32_16x16x32_f16: the V codes as f16 (a byte placed in
 //                  1024 + code + 128, less 1152), p times the block's scale as f16
 //                  hi + lo.  The scales enter through the exponent: each column keeps the
-//                  running maximum mw of score + e besides that of the score, and
-//                  its weights are 2^(score + e - mw) <= 1, whatever the sizes of V.
+//                  running maximum of score + e besides that of the score, and its
+//                  weights are 2^(score + e - that) <= 1, whatever the sizes of V.
 // Lane l of a tile: column c = l % 16, positions 16 (l / 16) .. + 15, all in one
 // block, so both exponents are a lane's own.
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNone = -1e30f;
+constexpr float kNone = -3e38f;
 
 // One value of q in fixed point: n = n2 2^16 + n1 2^8 + n0, three signed bytes, byte
 // `b` of a word each.
@@ -343,27 +343,24 @@ __device__ __forceinline__ h16x2 rest(h16x2 hi, float w0, float w1) {
   return h16x2{(_Float16)a, (_Float16)b};
 }
 
-// Two maxima over the lanes that share l % 16.  The exchanges of halves and rows
-// take two values at once.
-__device__ __forceinline__ void max_groups(float& x, float& y) {
-  auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
-  float v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));  // lower half: x, upper half: y
-  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  x = __uint_as_float(p[0]);
-  y = __uint_as_float(p[1]);
+// The maximum over the lanes that share l % 16.
+__device__ __forceinline__ float group_max(float x) {
+  auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
 
 // The running state of a wave's 16 columns.
 template <int HD>
 struct Column {
-  // before a column has seen a position, its maxima are far below every score's, and
-  // finite, so that the exponents' differences are numbers
-  float m = kNone, mw = kNone, l = 0.0f;  // l: of this lane's positions
+  // m: the largest score, far below every one and finite before the column has seen a
+  // position, so that differences are numbers; g: how far the largest score + e lies
+  // above m (a number of its own: next to a large score e would be lost)
+  float m = kNone, g = 0.0f, l = 0.0f;  // l: of this lane's positions
   float oc = 1.0f;
   bool grown = false;
-  f32x4 o[HD / 16];                               // 2^(14 - mw) O: dims 16 d + 4 r + i
+  f32x4 o[HD / 16];                               // 2^(14 - m - g) O: dims 16 d + 4 r + i
   __device__ __forceinline__ Column() {
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -419,17 +416,23 @@ struct Column {
     float f = ldexpf(sl2, ek);
     f = f < 1e-38f ? 1e-38f : f;
     mx = mx * f;
-    float mb = mx + ev;
-    max_groups(mx, mb);
-    const float mn = fmaxf(m, mx), wn = fmaxf(mw, mb);
+    const float mn = fmaxf(m, group_max(mx)), up = g + (m - mn), gn = fmaxf(up, group_max(ev + (mx - mn)));
     // a weight is p 2^gain: 2^14 puts hi and lo in f16's range, and below 2^-30 both are
     // zero whatever the gain, while p still counts in the sum
-    const float gain = fmaxf(ev + (mn - wn) + 14.0f, -30.0f), less = gain - mn;
+    const float gain = fmaxf(ev - gn + 14.0f, -30.0f), less = gain - mn;
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(sv[e], f, less);
+    // where the last place of the maximum counts, scores are rounded as it is
+    const bool coarse = fabsf(mn) > 0x1p20f && mn != kNone;
+    if (__ballot(coarse))
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = coarse ? (sv[e] * f - mn) + gain : x[e];
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-      const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], f, less));
-      const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], f, less));
+      const float w0 = __builtin_amdgcn_exp2f(x[e]);
+      const float w1 = __builtin_amdgcn_exp2f(x[e + 1]);
       sum += w0;
       sum += w1;
       const h16x2 hi = __builtin_bit_cast(h16x2, __builtin_amdgcn_cvt_pkrtz(w0, w1));
@@ -441,9 +444,9 @@ struct Column {
     }
     l = l * __builtin_amdgcn_exp2f(m - mn) + sum * __builtin_amdgcn_exp2f(-gain);
     m = mn;
-    grown = __ballot(wn != mw) != 0;
-    oc = __builtin_amdgcn_exp2f(mw - wn);
-    mw = wn;
+    grown = __ballot(gn != up) != 0;
+    oc = __builtin_amdgcn_exp2f(up - gn);
+    g = gn;
   }
   // O to the new maximum, where a column's has risen.
   __device__ __forceinline__ void rescale() {
@@ -457,7 +460,7 @@ struct Column {
   __device__ __forceinline__ void close() {
     l += xor16(l);
     l += xor32(l);
-    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mw - m - 14.0f) / l;
+    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(g - 14.0f) / l;
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) o[d] = o[d] * f;
   }

@@ -221,6 +221,28 @@ def test_attention_scores_of_any_size(hip, hd):
         b.check_attention(2, [0], [2], scale)
 
 
+@pytest.mark.parametrize("scale", [1e6, 1e8, 1e9, 1e20, 1e33, -1e9, -1e20, -1e33])
+@pytest.mark.parametrize("n", [2, 600])
+def test_attention_scores_past_f32s_steps(hip, n, scale):
+    """Scores whose last place in f32 is a factor of e and more, all of one sign:
+    which of the nearly greatest win is open, but the result is a weighted mean of
+    the values that a row sees (off by the roundings of the bound), never NaN."""
+    b = Both(hip, 1, 128, max_seq=1300, rope=None)
+    b.append([0], [1300], np.abs(b.rows(1300)), None)
+    q = np.abs(b.rng.standard_normal((n, 4 * 128))).astype(np.float32) * np.float32(scale)
+    got = b.gpu.attention(hip.Tensor.from_numpy(q), [0], [n]).data().reshape(n, 4, 128)
+    v = b.ref.values(0)[1][:, 0]
+    room = (1300 + 64) * 2.0 ** -24 * np.abs(v).max()
+    assert (got <= v.max(0) + room).all() and (got >= v.min(0) - room).all()
+    # one position far above the others: its value alone
+    k = np.full((65, 128), 1.0, np.float32)
+    k[40] = 2.0 if scale > 0 else 0.5
+    b.append([1], [65], k, b.rows(65))
+    got = b.gpu.attention(hip.Tensor.from_numpy(q[:2]), [1], [2]).data().reshape(2, 4, 128)
+    v = b.ref.values(1)[1][40, 0]
+    np.testing.assert_allclose(got, np.broadcast_to(v, got.shape), rtol=64 * 2.0 ** -24, atol=0)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("big,small", [(2.0 ** 60, 2.0 ** -60), (2.0 ** 15, 2.0 ** -15)])
 def test_attention_values_of_any_size(hip, hd, big, small):
