@@ -315,6 +315,77 @@ def test_attention_long(hip, length, counts):
         within(got[i:i + 1], *b.ref.attention(q[i:i + 1], [0], [1]))
 
 
+def check_sample(b, nq, slots, counts, scale=1.0):
+    """Attention of many rows, a few of each sequence against the reference."""
+    q = (b.rng.standard_normal((int(np.sum(counts)), nq * b.hd)) * scale).astype(np.float32)
+    got = b.gpu.attention(b.hip.Tensor.from_numpy(q), slots, counts).data()
+    assert np.isfinite(got).all()
+    row = 0
+    for s, n in zip(slots, counts):
+        length = b.gpu.length(s)
+        # the reference's rows one at a time: it takes the sequence as ending there
+        for i in sorted({0, n // 3, n - 1} & set(range(n))):
+            b.ref.truncate([s], [length - n + i + 1])
+            within(got[row + i:row + i + 1], *b.ref.attention(q[row + i:row + i + 1], [s], [1]))
+        b.ref.truncate([s], [length])
+        row += n
+    return q, got
+
+
+# (query heads, KV heads, head_dim, page, lengths, rows): enough columns for the kernel
+# of 64 of them, 96 for each of 256 CUs, in whole tiles and with a rest, behind earlier
+# positions and from the first on
+MANY = [(32, 8, 128, 64, [1000], [800]), (32, 8, 128, 32, [777], [777]), (16, 16, 64, 128, [1601], [1600]),
+        (64, 2, 128, 256, [451], [387]), (32, 8, 64, 32, [500, 1, 400, 333], [500, 1, 400, 16]),
+        (32, 8, 128, 64, [300, 700, 65, 63, 1025], [300, 500, 65, 0, 1])]
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page,lens,counts", MANY)
+def test_attention_many_columns(hip, nq, nkv, hd, page, lens, counts):
+    b = Both(hip, nkv, hd, page=page, max_seq=2048)
+    slots = list(range(len(lens)))[::-1]
+    b.append(slots, lens)
+    check_sample(b, nq, slots, counts)
+
+
+def test_attention_many_columns_scores_of_any_size(hip):
+    """As for few columns: zeros, peaked softmaxes, one sign past f32's steps."""
+    b = Both(hip, 8, 128, max_seq=1024, rope=None)
+    b.append([0], [850], np.abs(b.rows(850)), None)
+    for scale in (0.0, 30.0, 1e4):
+        check_sample(b, 32, [0], [800], scale)
+    v = b.ref.values(0)[1]
+    room = (1024 + 64) * 2.0 ** -24 * np.abs(v).max()
+    for scale in (1e6, 1e9, 1e33, -1e9, -1e33):
+        q = np.abs(b.rng.standard_normal((800, 32 * 128))).astype(np.float32) * np.float32(scale)
+        got = b.gpu.attention(hip.Tensor.from_numpy(q), [0], [800]).data().reshape(800, 8, 4, 128)
+        assert (got <= v.max(0)[None, :, None] + room).all() and (got >= v.min(0)[None, :, None] - room).all()
+
+
+def test_attention_many_columns_not_finite_and_same_bits(hip):
+    b = Both(hip, 8, 128, max_seq=1024)
+    b.append([0, 1], [850, 40])
+    q, clean = check_sample(b, 32, [0, 1], [800, 1])
+    np.testing.assert_array_equal(b.gpu.attention(hip.Tensor.from_numpy(q), [0, 1], [800, 1]).data(), clean)
+    bad = np.zeros((801, 32, 128), bool)
+    for row, head, x in ((0, 3, np.nan), (517, 31, np.inf), (799, 0, -np.inf), (800, 7, np.nan)):
+        q[row, 128 * head + 5] = x
+        bad[row, head] = True
+    bad = bad.reshape(801, -1)
+    got = b.gpu.attention(hip.Tensor.from_numpy(q), [0, 1], [800, 1]).data()
+    assert np.isnan(got[bad]).all()
+    np.testing.assert_array_equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("lens,counts", [([9000] + [40] * 70, [1] * 71), ([9000, 300, 300], [16, 300, 300])])
+def test_attention_one_sequence_outlasts_the_others(hip, lens, counts):
+    """A batch that fills the chip, with one long sequence whose tiles are split."""
+    b = Both(hip, 8, 64, seqs=len(lens), max_seq=9216)
+    slots = list(range(len(lens)))
+    b.append(slots, lens)
+    check_sample(b, 64, slots, counts)
+
+
 def test_same_call_same_bits(hip):
     """No result depends on the order workgroups end in."""
     b = Both(hip, 8, 128, seqs=4, max_seq=1000)
