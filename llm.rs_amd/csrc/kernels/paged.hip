@@ -62,9 +62,13 @@ __device__ __forceinline__ Seq find_seq(const PagedSeqs& s, int item) {
   return q;
 }
 
-// The pool block that holds block `b` of a slot.
+// The pool block that holds block `b` of a slot, the same for all lanes.  The table is
+// read through the scalar cache: a vector load would be waited for together with the
+// codes that are on their way (no kernel here writes the table that it reads).
 __device__ __forceinline__ int pool_block(const PagedPool& p, int slot, int b) {
-  return (__builtin_amdgcn_readfirstlane(p.table[(size_t)slot * p.stride + (b >> p.shift)]) << p.shift) + (b & ((1 << p.shift) - 1));
+  const int* at = p.table + (size_t)slot * p.stride + (b >> p.shift);
+  const int page = *(const __attribute__((address_space(4))) int*)(uintptr_t)at;
+  return (page << p.shift) + (b & ((1 << p.shift) - 1));
 }
 
 // The smallest e in [kPagedExpMin, kPagedExpMax] with amax <= 127 * 2^e: amax =
@@ -317,7 +321,6 @@ __device__ __forceinline__ float row_scale(float scale, int ex, bool odd) {
 
 // Eight codes of V (positions of one half of a lane's 16) as f16.
 __device__ __forceinline__ h16x8 v_half(unsigned w0, unsigned w1) {
-  asm("" : "+v"(w0), "+v"(w1));  // words: else the compiler carries them to here byte by byte
   const h16x2 less = {(_Float16)-1152.0f, (_Float16)-1152.0f};
   h16x8 v;
 #pragma unroll
@@ -359,7 +362,6 @@ struct Column {
   // above m (a number of its own: next to a large score e would be lost)
   float m = kNone, g = 0.0f, l = 0.0f;  // l: of this lane's positions
   float oc = 1.0f;
-  bool grown = false;
   f32x4 o[HD / 16];                               // 2^(14 - m - g) O: dims 16 d + 4 r + i
   __device__ __forceinline__ Column() {
 #pragma unroll
@@ -444,13 +446,12 @@ struct Column {
     }
     l = l * __builtin_amdgcn_exp2f(m - mn) + sum * __builtin_amdgcn_exp2f(-gain);
     m = mn;
-    grown = __ballot(gn != up) != 0;
     oc = __builtin_amdgcn_exp2f(up - gn);
     g = gn;
   }
   // O to the new maximum, where a column's has risen.
   __device__ __forceinline__ void rescale() {
-    if (grown) {
+    if (__ballot(oc != 1.0f)) {
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) o[d] = o[d] * oc;
     }
@@ -500,7 +501,7 @@ struct Place {
 __device__ __forceinline__ Place place_of(const PagedAttnArgs& a, const Item& t, int t0) {
   const int b = t0 / kBlk, nkv = a.pool.nkv;
   const int b0 = pool_block(a.pool, t.q.slot, b);
-  const int b1 = (b + 1) * kBlk < t.q.pos ? pool_block(a.pool, t.q.slot, b + 1) : b0;
+  const int b1 = pool_block(a.pool, t.q.slot, (b + 1) * kBlk < t.q.pos ? b + 1 : b);
   return {((size_t)b0 * nkv + t.head) * 2, ((size_t)b1 * nkv + t.head) * 2};
 }
 
@@ -630,8 +631,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
   u32x4 vv[ND];
   unsigned exps = 0;  // of the lane's positions: K, V
   const uint8_t* vp = nullptr;
-  auto fetch_k = [&](int t0) {
-    const Place p = place_of(a, t, t0);
+  auto fetch_k = [&](const Place& p) {
     const size_t uk = c < 8 ? p.u0 : p.u1, uv = r < 2 ? p.u0 : p.u1;
     exps = *(const uint16_t*)(a.pool.exps + uv);
     const uint8_t* kp = a.pool.codes + uk * BYTES + r * 128 + (c & 7) * 16;
@@ -647,7 +647,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
   };
   int t0 = t.from + 64 * wave;
   if (t0 < t.to) {
-    fetch_k(t0);
+    fetch_k(place_of(a, t, t0));
     fetch_v();
   }
   __builtin_amdgcn_sched_barrier(0);
@@ -711,13 +711,15 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
   for (; t0 < t.to; t0 += STEP) {
     const int ek = (int8_t)(exps & 255);
     const float ev = (float)(int8_t)(exps >> 8);
+    const bool more = t0 + STEP < t.to;
+    const Place next = place_of(a, t, more ? t0 + STEP : t0);
     float sv[16];
     asm volatile("" ::: "memory");  // q is read again for every tile: its registers are worth more
     Column<HD>::template scores<4>([&](int b, int s) { return kk[b][s]; },
                                     [&](int k, int s) { return sq[(k * S + s) * LLMRS_WAVE + lane]; }, sv);
     if (t0 + 63 > lowest) Column<HD>::hide(limit - t0 - 16 * r, sv);
     __builtin_amdgcn_sched_barrier(0);
-    if (t0 + STEP < t.to) fetch_k(t0 + STEP);
+    if (more) fetch_k(next);
     __builtin_amdgcn_sched_barrier(0);
     h16x8 ph[2], pl[2];
     x.weigh(sv, sl2, ek, ev, ph, pl);
@@ -741,7 +743,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (t0 + STEP < t.to) fetch_v();
+    if (more) fetch_v();
     __builtin_amdgcn_sched_barrier(0);
   }
   // the waves' results, in order; wave 0 has the sum
@@ -884,7 +886,10 @@ __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) put_bytes(odd ? 0.0f : v[s][4 * k + b], ex, b, w);
 #pragma unroll
-        for (int n = 0; n < 3; ++n) qb[n][s][k] = (int)w[n];
+        for (int n = 0; n < 3; ++n) {
+          asm("" : "+v"(w[n]));  // words: else the loop puts them together again for every tile
+          qb[n][s][k] = (int)w[n];
+        }
       }
     sl2 = row_scale(a.scale, ex, odd);
   }
