@@ -123,6 +123,11 @@ constexpr int block_threads(int hd) { return 2 * hd; }
 // Older codes are loaded and, where the new rows raise the exponent, rounded to the
 // new step.  K is rotated in 64 bits (the products of f32 values are exact there), so
 // a code does not depend on how a sum was rounded.
+// Bound by memory for prompts: 4 x 2048 rows of 8 heads x 128 in 18.0 us, 84 MB at 4.7
+// TB/s (a copy reaches 5.1); with the codes passed through LDS byte by byte it was about
+// 25.  A decode step of 64 sequences takes 5.1 us and one row 3.3, a chain of
+// dependent accesses (words, page, exponent, codes); 64-bit work where no new row is made
+// it 6.8.
 template <int HD>
 __device__ __forceinline__ void append_block(const PagedRowsArgs& a) {
   constexpr int MID = HD / 2, BYTES = kBlk * HD, LANES = MID / 4, WAVES = block_threads(HD) / LLMRS_WAVE;
@@ -237,6 +242,7 @@ extern "C" __global__ __launch_bounds__(block_threads(64)) void paged_append_hd6
 extern "C" __global__ __launch_bounds__(block_threads(128)) void paged_append_hd128(PagedRowsArgs a) { append_block<128>(a); }
 
 // Reads one block's rows of a range back as f32; a thread has the codes of the append.
+// Bound by memory: 4 x 2048 rows of 8 heads x 128 in 18.2 us, 84 MB at 4.6 TB/s.
 template <int HD>
 __device__ __forceinline__ void read_block(const PagedRowsArgs& a) {
   constexpr int MID = HD / 2, BYTES = kBlk * HD, LANES = MID / 4;
@@ -612,6 +618,14 @@ __device__ __forceinline__ void join_splits(const PagedAttnArgs& a, const Item& 
 // 16 columns: the four waves take every fourth tile of the split each, with
 // the codes straight from the cache, and merge through LDS.  q is prepared by all
 // of them together, 16 lanes a column, while the first tile is on its way.
+// Bound by the stream of codes where they are many: 64 sequences of 1000 to 4000
+// positions, 331 MB, in 57 us (5.8 TB/s; a stream that only reads reaches 7.1); 8 heads
+// of one sequence behind 32 k positions, 67 MB, in 18.7 us, of which the join of 32
+// splits is about 4 (one CU reads their results at some 45 GB/s) and start and end 4.
+// Short contexts are a chain of dependent accesses: 8 us for 512 positions.  32 and 48
+// columns per workgroup read the cache less often and were slower at every size tried (16
+// sequences, 5 rows of 4 heads behind 2100 positions: 22.8 us with 16, 27.5 and 48.4), as
+// were three waves per SIMD (57 us became 60; registers spill).
 template <int HD>
 __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
   constexpr int S = HD / 64, ND = HD / 16, MID = HD / 2, BYTES = kBlk * HD, WP = 4, COLS = 16, STEP = 64 * WP;
@@ -783,6 +797,11 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
 // More columns: each wave has 16 of its own and takes every tile of the split.  The
 // workgroup brings a tile into LDS once, V already as f16, while the one before is
 // computed.
+// Bound by issue: a tile of 16 columns is 56 matrix instructions (900 cycles) and about
+// 240 others (1150), and the two overlap little although three waves share a SIMD; 2048
+// rows of 32 heads behind 2048 positions take 183 to 200 us, 103 GFLOP of the formula.
+// 128 columns in eight waves, raised priority of the matrix phases (208 us), and the
+// next tile's scores taken before this one's weights were no faster.
 template <int HD>
 __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
   constexpr int S = HD / 64, ND = HD / 16, MID = HD / 2, BYTES = kBlk * HD, COLS = 64, T = kThreads;

@@ -220,6 +220,9 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const uns
 // waiting; the sums move with device-scope stores and loads) draws, one wave of it
 // alone: the slice in which the running sum crosses, and the id in that slice.  Its
 // answer goes straight to the host's memory, where the caller waits for the stamps.
+// Bound by latency (words, drafted ids, row, sums, ticket, sums, slice): 5.7 us for one
+// sequence of 32000 ids, 8.3 us for 32 of 128256 with drafts' probabilities (33 MB);
+// tickets next to each other in memory made that 34.
 extern "C" __global__ __launch_bounds__(kThreads) void verify_rows(VerifyArgs a) {
   const int i = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(wave_id());
   const Row r = examine(a, i);
