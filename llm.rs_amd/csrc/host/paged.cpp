@@ -169,17 +169,17 @@ struct AttnKind {
 };
 constexpr AttnKind kFew{"few", 16, 256}, kMany{"many", 64, 64};
 // Columns per CU from which the kernel of 64 is the faster: with 64 of them (512 rows
-// of 32 heads behind 500 positions) 29.3 us against 27.4, with 100 (4 x 200 rows
-// behind 1000) 36.1 against 39.3, with 128 45.2 against 46.9, with 256 (4 x 512 rows) 29.5
-// against 55.2 and with 256 behind 2048 positions 194 against 277.
+// of 32 heads behind 500 positions) 33.1 us against 28.2, with 96 (768 rows behind 1000)
+// 50.1 against 51.0, with 100 (4 x 200 rows behind 1000) 43.4 against 52.7, with 256 (4 x
+// 512 rows) 35.4 against 67.3 and with 256 behind 2048 positions 185 against 243.
 constexpr long kManyColumns = 96;
 
-// Units of a split.  One workgroup per CU: a second one has each wait for the other's
-// loads, and doubles what is joined (8 sequences of 4000 positions: 16.7 us either way;
-// one of 2048 with 32 columns a head 13.8 us with one, 16.3 with two).  Where that
-// would split nothing though CUs stand half empty behind long caches, two (16
-// sequences of 2100, two workgroups a head: 19.5 us against 23.8).  A batch that fills
-// the chip unsplit keeps whole sequences but for the ones that would outlast it.
+// Units of a split.  One workgroup per CU: a second one doubles what is joined for
+// little (8 sequences of 4000 positions: 16.7 us with one, 16.4 with two; 64 of 1000 to
+// 4000: 57 and 73).  Where that would split nothing though CUs stand half empty, two: they
+// even out lengths (16 sequences of 500 to 2100 positions, two workgroups a head: 17.7 us
+// against 20.1; of equal lengths 23.9 against 22.3).  A batch that fills the chip unsplit
+// keeps whole sequences but for the ones that would outlast it.
 int split_units(const std::vector<Part>& parts, long heads, int n_rep, const AttnKind& kind, long cus) {
   long units = 0, whole = 0;
   int longest = 0;

@@ -797,11 +797,13 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
 // More columns: each wave has 16 of its own and takes every tile of the split.  The
 // workgroup brings a tile into LDS once, V already as f16, while the one before is
 // computed.
-// Bound by issue: a tile of 16 columns is 56 matrix instructions (900 cycles) and about
-// 240 others (1150), and the two overlap little although three waves share a SIMD; 2048
-// rows of 32 heads behind 2048 positions take 183 to 200 us, 103 GFLOP of the formula.
-// 128 columns in eight waves, raised priority of the matrix phases (208 us), and the
-// next tile's scores taken before this one's weights were no faster.
+// Bound by issue: a tile of 16 columns is 56 matrix instructions, 17 exp2 and about 220
+// others, which in a loop of two or three waves per SIMD cost 8, 9.6 and 4.4 cycles of
+// it: 1590 of the 2175 that a tile takes.  2048 rows of 32 heads behind 2048 positions
+// are 183 to 200 us, 103 GFLOP of the formula.  No faster were 128 columns in eight waves,
+// 32 columns per wave (346 us: registers spill; 64 dims: 150 against 136), the next tile's
+// scores among this one's weights (205 to 215) and raised priority of the matrix
+// instructions (208).
 template <int HD>
 __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
   constexpr int S = HD / 64, ND = HD / 16, MID = HD / 2, BYTES = kBlk * HD, COLS = 64, T = kThreads;
