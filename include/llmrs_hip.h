@@ -448,7 +448,9 @@ int llmrs_paged_read(llmrs_paged* p, const int32_t* slots, const int32_t* starts
  * same shape.  Row t of a sequence of length L and count c sits at position p =
  * L - c + t: softmax over the positions up to p of (rotated q . K) / sqrt(head_dim),
  * times V.  Query head h reads KV head h / (query heads / KV heads).  A q row
- * with a NaN or an infinity gives NaN in that head alone. */
+ * with a NaN or an infinity gives NaN in that head alone.  The same call gives the
+ * same bits; how long sequences are split follows from all of a call's, so a
+ * sequence's last bits may change with its company. */
 int llmrs_paged_attention(llmrs_paged* p, const llmrs_tensor* q, const int32_t* slots, const int32_t* counts, size_t n,
                           llmrs_tensor** out);
 

@@ -15,6 +15,7 @@ import ctypes as C
 import enum
 import os
 from dataclasses import dataclass
+from operator import index
 from pathlib import Path
 
 import numpy as np
@@ -298,6 +299,8 @@ class Tensor:
         info = getattr(x, "__cuda_array_interface__", None)
         if info is None:
             raise LlmrsError(E_INVALID, "from_device: not an array in device memory")
+        if info.get("mask") is not None:
+            raise LlmrsError(E_INVALID, "from_device: masked arrays have no values everywhere")
         if info["typestr"] != "<f4":
             raise LlmrsError(E_DTYPE, f"from_device: f32 values, not {info['typestr']}")
         shape = tuple(info["shape"]) or (1,)
@@ -758,10 +761,22 @@ def _vec(a, dtype) -> np.ndarray:
     """A flat contiguous array; one that is, as it is."""
     if type(a) is np.ndarray and a.dtype is dtype and a.ndim == 1 and a.flags.c_contiguous:
         return a
-    return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
+    x = np.asarray(a)
+    out = np.ascontiguousarray(x, dtype=dtype).reshape(-1)
+    if dtype is _I32 and x.size and (x.dtype.kind not in "iu" or (out != x.reshape(-1)).any()):
+        raise LlmrsError(E_INVALID, "whole numbers of 32 bits are required")
+    return out
 
 
 _I32, _F32 = np.dtype(np.int32), np.dtype(np.float32)
+
+
+def _int(x) -> int:
+    """A whole number as a C int (ctypes would keep its low bits)."""
+    x = index(x)
+    if not -2**31 <= x < 2**31:
+        raise LlmrsError(E_RANGE, f"{x} is not a number of 32 bits")
+    return x
 
 
 def _pair(a, b, what: str):
@@ -786,7 +801,7 @@ class HipPagedCache:
         elif rope is not None:
             theta = float(rope)
         self._width = n_kv_heads * head_dim
-        self.cfg = PagedConfig(n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_seq, theta)
+        self.cfg = PagedConfig(*(_int(x) for x in (n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_seq)), theta)
         h = C.c_void_p()
         _check(lib().llmrs_paged_create(C.byref(self.cfg), _ptr(cos), _ptr(sin), C.byref(h)))
         self._h = h
@@ -805,15 +820,15 @@ class HipPagedCache:
     def map(self, slot: int, pages) -> None:
         """Adds pages at the end of a slot's."""
         pages = _vec(pages, _I32)
-        _check(lib().llmrs_paged_map(self._h, int(slot), _ref(pages), pages.size))
+        _check(lib().llmrs_paged_map(self._h, _int(slot), _ref(pages), pages.size))
 
     def release(self, slot: int) -> None:
         """Ends a slot's sequence and frees its pages."""
-        _check(lib().llmrs_paged_release(self._h, int(slot)))
+        _check(lib().llmrs_paged_release(self._h, _int(slot)))
 
     def length(self, slot: int) -> int:
         n = C.c_int32()
-        _check(lib().llmrs_paged_length(self._h, int(slot), C.byref(n)))
+        _check(lib().llmrs_paged_length(self._h, _int(slot), C.byref(n)))
         return int(n.value)
 
     def truncate(self, slots, lengths) -> None:

@@ -476,6 +476,29 @@ def test_verify(hip, vocab, given, counts):
     check_verify(hip, target, ids, counts, uniform(rng, n), uniform(rng, len(counts)), draft)
 
 
+@pytest.mark.parametrize("given", [True, False])
+def test_verify_vocabularies_past_a_wave_of_sums(hip, given):
+    """More than 512 slices of 512 ids; draws in each part."""
+    rng = np.random.default_rng(8)
+    V, counts = 512 * 1024 + 77, [1, 0, 2]
+    target = probabilities(rng, 6, V)
+    draft = probabilities(rng, 3, V) if given else None
+    ids = rng.integers(0, V, 3)
+    for x in (0.0, 0.2, 0.51, 0.75, 0.999, 1.0 - 2.0 ** -24):
+        check_verify(hip, target, ids, counts, uniform(rng, 3), np.full(3, x, np.float32), draft)
+        check_verify(hip, target, ids, counts, np.zeros(3, np.float32), np.full(3, x, np.float32), draft)
+
+
+def test_verify_answers_past_the_host_buffer(hip):
+    """So many sequences that the answer comes through device memory."""
+    rng = np.random.default_rng(9)
+    n, V = 44000, 5
+    counts = rng.integers(0, 2, n).astype(np.int32)
+    rows = int(counts.sum())
+    target = probabilities(rng, rows + n, V, 1.0)
+    check_verify(hip, target, rng.integers(0, V, rows), counts, uniform(rng, rows), uniform(rng, n))
+
+
 def test_verify_many_sequences(hip):
     rng = np.random.default_rng(5)
     counts = [int(c) for c in rng.integers(0, 7, 300)]

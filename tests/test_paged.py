@@ -76,6 +76,29 @@ def test_mapping_pages():
     refused(lh.E_RANGE, c.release, 7)
 
 
+@pytest.mark.parametrize("bad", [[2 ** 32], np.array([2 ** 32]), np.array([-2 ** 32]), np.array([2 ** 31], np.uint32),
+                                 [0.5], np.array([0.0]), np.array([True])])
+def test_numbers_that_are_no_slots(bad):
+    """Wider numbers are not cut to 32 bits, and fractions not rounded."""
+    c = cache()
+    c.map(0, [0])
+    for slots, counts in ((bad, [0]), ([0], bad)):
+        refused(lh.E_INVALID, c.truncate, slots, counts)
+        refused(lh.E_INVALID, c.append, None, None, slots, counts)
+        refused(lh.E_INVALID, c.attention, None, slots, counts)
+        refused(lh.E_INVALID, c.read, slots, [0], counts)
+    refused(lh.E_INVALID, c.read, [0], bad, [0])
+    refused(lh.E_INVALID, c.map, 1, bad)
+    refused(lh.E_INVALID, lh.verify_drafts, None, bad, [1], [0.5], [0.5])
+    refused(lh.E_INVALID, lh.verify_drafts, None, [0], bad, [0.5], [0.5])
+    for call in (lambda s: c.map(s, [1]), c.release, c.length, lambda n: cache(n_pages=n), lambda n: cache(max_seq=n)):
+        refused(lh.E_RANGE, call, 2 ** 32)
+        with pytest.raises(TypeError):
+            call(0.5)
+    assert c.length(0) == 0 and c.length(1) == 0
+    c.truncate(np.array([0], np.int64), [0])
+
+
 def test_lengths_only_shrink():
     c = cache()
     refused(lh.E_RANGE, c.truncate, [0], [1])
