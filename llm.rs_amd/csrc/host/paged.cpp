@@ -173,6 +173,11 @@ constexpr AttnKind kFew{"few", 16, 256}, kMany{"many", 64, 64};
 // 50.1 against 51.0, with 100 (4 x 200 rows behind 1000) 43.4 against 52.7, with 256 (4 x
 // 512 rows) 35.4 against 67.3 and with 256 behind 2048 positions 185 against 243.
 constexpr long kManyColumns = 96;
+// Positions x head_dim up to which a sequence is not split: joining takes 2.7 us, 256
+// more positions in one workgroup 1.05 us with 64 dims and 2 with 128 (one row behind 512
+// positions of 64 dims 7.4 us whole, 8.2 in three; behind 300 of 128 8.4 and 9.4; behind
+// 1000 of 128 11.8 and 9.6).
+constexpr long kWhole = 65536;
 
 // Units of a split.  One workgroup per CU: a second one doubles what is joined for
 // little (8 sequences of 4000 positions: 16.7 us with one, 16.4 with two; 64 of 1000 to
@@ -180,7 +185,7 @@ constexpr long kManyColumns = 96;
 // even out lengths (16 sequences of 500 to 2100 positions, two workgroups a head: 17.7 us
 // against 20.1; of equal lengths 23.9 against 22.3).  A batch that fills the chip unsplit
 // keeps whole sequences but for the ones that would outlast it.
-int split_units(const std::vector<Part>& parts, long heads, int n_rep, const AttnKind& kind, long cus) {
+int split_units(const std::vector<Part>& parts, long heads, int n_rep, int hd, const AttnKind& kind, long cus) {
   long units = 0, whole = 0;
   int longest = 0;
   auto tiles = [&](const Part& s) { return heads * ((s.rows * (long)n_rep + kind.cols - 1) / kind.cols); };
@@ -191,6 +196,7 @@ int split_units(const std::vector<Part>& parts, long heads, int n_rep, const Att
   }
   const long slots = 2 * whole > cus && whole <= cus ? 2 * cus : cus;
   const int most = (longest + kind.unit - 1) / kind.unit;
+  if ((long)most * kind.unit * hd <= kWhole) return most;
   int per = (int)std::max<long>((units + slots - 1) / slots, (most + kPagedMaxSplits - 1) / kPagedMaxSplits);
   for (; whole <= slots && per < most; ++per) {
     long groups = 0;
@@ -212,7 +218,7 @@ void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, 
   a.nq = (int)(q->dims[1] / (size_t)hd);
   a.scale = 1.0f / std::sqrt((float)hd);
   const int n_rep = a.nq / nkv, unit = kind.unit;
-  const int per = split_units(parts, nkv, n_rep, kind, ctx().num_cus);
+  const int per = split_units(parts, nkv, n_rep, hd, kind, ctx().num_cus);
   a.chunk = per * unit;
   std::vector<int> items;
   bool split = false;
