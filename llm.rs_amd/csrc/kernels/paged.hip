@@ -511,26 +511,25 @@ __device__ __forceinline__ Place place_of(const PagedAttnArgs& a, const Item& t,
   return {((size_t)b0 * nkv + t.head) * 2, ((size_t)b1 * nkv + t.head) * 2};
 }
 
-// A column's result, or the split's part of it.
+// A column's result in dims 16 d + 4 r .. of lane group r, or the split's part of it.
 template <int HD>
-__device__ __forceinline__ void put_column(const PagedAttnArgs& a, const Item& t, int cols, int local, const Column<HD>& x) {
+__device__ __forceinline__ void put_dims(const PagedAttnArgs& a, const Item& t, int cols, int local, int d, f32x4 o) {
   const int r = lane_id() >> 4, col = t.tile * cols + local;
   if (col >= t.n_col) return;
   if (t.n_split == 1) {
-    float* dst = out_row(a, t, col, HD);
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d) *(f32x4*)(dst + 16 * d + 4 * r) = x.o[d];
-    return;
-  }
-  const size_t unit = ((size_t)t.item * a.pool.nkv + t.head) * cols;
-#pragma unroll
-  for (int d = 0; d < HD / 16; ++d)
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(dev_u32x4, x.o[d]), dev_rsrc(a.part_o + unit * HD),
+    *(f32x4*)(out_row(a, t, col, HD) + 16 * d + 4 * r) = o;
+  } else {
+    const size_t unit = ((size_t)t.item * a.pool.nkv + t.head) * cols;
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(dev_u32x4, o), dev_rsrc(a.part_o + unit * HD),
                                            (local * HD + 16 * d + 4 * r) * 4, 0, kSc1);
-  if (r == 0) {
-    __builtin_amdgcn_raw_buffer_store_b64(dev_u32x2{__float_as_uint(x.m), __float_as_uint(x.l)}, dev_rsrc(a.part_ml + unit * 2),
-                                          local * 8, 0, kSc1);
   }
+}
+// The maximum and sum of a split's column.
+__device__ __forceinline__ void put_sum(const PagedAttnArgs& a, const Item& t, int cols, int local, float m, float l) {
+  if (t.n_split == 1 || lane_id() >= 16 || t.tile * cols + local >= t.n_col) return;
+  const size_t unit = ((size_t)t.item * a.pool.nkv + t.head) * cols;
+  __builtin_amdgcn_raw_buffer_store_b64(dev_u32x2{__float_as_uint(m), __float_as_uint(l)}, dev_rsrc(a.part_ml + unit * 2), local * 8,
+                                        0, kSc1);
 }
 
 // One wave joins the splits of U columns from `col` on (those past the tile's last are
@@ -760,7 +759,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
     if (more) fetch_v();
     __builtin_amdgcn_sched_barrier(0);
   }
-  // the waves' results, in order; wave 0 has the sum
+  // the waves' results, in order; each wave adds them in dims of its own
   x.close();
 #pragma unroll
   for (int d = 0; d < ND; ++d) *(f32x4*)(so + (wave * 16 + c) * HD + 16 * d + 4 * r) = x.o[d];
@@ -769,28 +768,22 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
     sm[(wave * 16 + c) * 2 + 1] = x.l;
   }
   __syncthreads();
-  if (wave == 0) {
-    float M = x.m;
+  float M = sm[c * 2], L = 0.0f, cw[WP];
 #pragma unroll
-    for (int w = 1; w < WP; ++w) M = fmaxf(M, sm[(w * 16 + c) * 2]);
-    float L = 0.0f, cw[WP];
+  for (int w = 1; w < WP; ++w) M = fmaxf(M, sm[(w * 16 + c) * 2]);
 #pragma unroll
-    for (int w = 0; w < WP; ++w) {
-      cw[w] = __builtin_amdgcn_exp2f(sm[(w * 16 + c) * 2] - M) * sm[(w * 16 + c) * 2 + 1];
-      L += cw[w];
-    }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int w = 0; w < WP; ++w) acc = acc + *(const f32x4*)(so + (w * 16 + c) * HD + 16 * d + 4 * r) * (cw[w] * inv);
-      x.o[d] = acc;
-    }
-    x.m = M;
-    x.l = L;
-    put_column<HD>(a, t, COLS, c, x);
+  for (int w = 0; w < WP; ++w) {
+    cw[w] = __builtin_amdgcn_exp2f(sm[(w * 16 + c) * 2] - M) * sm[(w * 16 + c) * 2 + 1];
+    L += cw[w];
   }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  for (int d = wave; d < ND; d += WP) {
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < WP; ++w) acc = acc + *(const f32x4*)(so + (w * 16 + c) * HD + 16 * d + 4 * r) * (cw[w] * inv);
+    put_dims<HD>(a, t, COLS, c, d, acc);
+  }
+  if (wave == 0) put_sum(a, t, COLS, c, M, L);
   join_splits<HD>(a, t, COLS, &ticket);
 }
 
@@ -956,7 +949,9 @@ __device__ __forceinline__ void attend_many(const PagedAttnArgs& a) {
     __syncthreads();
   }
   x.close();
-  put_column<HD>(a, t, COLS, wave * 16 + c, x);
+#pragma unroll
+  for (int d = 0; d < ND; ++d) put_dims<HD>(a, t, COLS, wave * 16 + c, d, x.o[d]);
+  put_sum(a, t, COLS, wave * 16 + c, x.m, x.l);
   join_splits<HD>(a, t, COLS, &ticket);
 }
 
