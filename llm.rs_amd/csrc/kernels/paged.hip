@@ -619,7 +619,7 @@ __device__ __forceinline__ void join_splits(const PagedAttnArgs& a, const Item& 
 // of them together, 16 lanes a column, while the first tile is on its way.
 // Bound by the stream of codes where they are many: 64 sequences of 1000 to 4000
 // positions, 331 MB, in 57 us (5.8 TB/s; a stream that only reads reaches 7.1); 8 heads
-// of one sequence behind 32 k positions, 67 MB, in 18.7 us, of which the join of 32
+// of one sequence behind 32 k positions, 67 MB, in 18.1 us, of which the join of 32
 // splits is about 4 (one CU reads their results at some 45 GB/s) and start and end 4.
 // Short contexts are a chain of dependent accesses: 7.5 us for 512 positions.  32 and 48
 // columns per workgroup read the cache less often and were slower at every size tried (16

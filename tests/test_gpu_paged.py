@@ -198,10 +198,10 @@ def test_attention_several_rows(hip, nq, nkv, hd, page, lens, counts):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
-def test_attention_mixed_batch(hip, hd):
-    """A prompt, drafts and single tokens in one call, over many sequences (more
-    than a launch's own arguments hold)."""
-    n = 130
+@pytest.mark.parametrize("n", [96, 97, 130, 300])
+def test_attention_mixed_batch(hip, hd, n):
+    """A prompt, drafts and single tokens in one call, over many sequences: as many
+    as a launch's own arguments hold (96), and more."""
     b = Both(hip, 2, hd, seqs=n, max_seq=200, seed=3)
     lens = [1 + (37 * i) % 90 for i in range(n)]
     lens[7], lens[60] = 150, 120
