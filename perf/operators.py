@@ -227,15 +227,13 @@ def _verify_inputs(case, seed):
 def prepare(case, seed):
     s = _verify_inputs(case, seed) if case["op"] == "verify" else _cache_inputs(case, seed)
     if own:
-        # the handles that a program on this framework holds
+        # the handles that a program on this framework holds: the library, the batch's slots and
+        # lengths, the cache with what it holds (tensors and numbers are handed over in the pass)
         sys.path.insert(0, str(Path.cwd() / "llm.rs_amd"))
         lh = s["lh"] = importlib.import_module("llmrs_hip")
         lh.init(0)
-        device = lambda t: lh.Tensor.from_device(t.contiguous())  # noqa: E731
         if case["op"] == "verify":
-            s["own"] = {"target": device(s["target"]), "draft": None if s["draft"] is None else device(s["draft"]),
-                        "ids": s["ids"].cpu().numpy(), "accept": s["accept"].cpu().numpy(), "draw": s["draw"].cpu().numpy(),
-                        "counts": np.array(s["drafts"], np.int32)}
+            s["own"] = {"counts": np.array(s["drafts"], np.int32)}
             return s
         nq, nkv, hd = HEADS[case["heads"]]
         n = case["seqs"]
@@ -244,13 +242,19 @@ def prepare(case, seed):
         for i, pages in enumerate(s["table"]):
             cache.map(i, pages)
         slots, held = np.arange(n, dtype=np.int32), np.array(s["held"], np.int32)
-        if held.sum():
-            kept = torch.arange(s["blocks"].shape[1] * BLOCK, device=DEV) < s["n_held"][:, None]
-            k, v = (_values(s, x).reshape(n, -1, nkv * hd)[kept] for x in "kv")
-            cache.append(device(k), device(v), slots, held, rotate=False)
         past, rows = np.array(s["past"], np.int32), np.array(s["rows"], np.int32)
+
+        def cached(starts, ends):  # what the cache holds of these positions
+            at = torch.arange(s["blocks"].shape[1] * BLOCK, device=DEV)
+            kept = (at >= _ints(starts)[:, None]) & (at < _ints(ends)[:, None])
+            return [lh.Tensor.from_device(_values(s, x).reshape(n, -1, nkv * hd)[kept].contiguous()) for x in "kv"]
+
+        if held.sum():
+            cache.append(*cached([0] * n, s["held"]), slots, held, rotate=False)
         s["own"] = {"cache": cache, "slots": slots, "rows": rows, "past": past, "from": past // BLOCK * BLOCK,
-                    "back": past % BLOCK + rows, "q": device(s["q"]), "k": device(s["new_k"]), "v": device(s["new_v"])}
+                    "older": past % BLOCK, "back": past % BLOCK + rows}
+        if case["op"] == "append":
+            s["own"]["begun"] = cached((past // BLOCK * BLOCK).tolist(), s["past"])
     return s
 
 
@@ -258,24 +262,33 @@ def prepare(case, seed):
 def run(s):
     op = s["case"]["op"]
     if own:
-        return {"append": _own_append, "attention": _own_attention, "verify": _own_verify}[op](s["own"], s["lh"])
+        return {"append": _own_append, "attention": _own_attention, "verify": _own_verify}[op](s, s["own"], s["lh"])
     return {"append": _append, "attention": _attention, "verify": _verified}[op](s)
 
 
-def _own_append(o, lh):
+def _own_append(s, o, lh):
     c = o["cache"]
-    c.truncate(o["slots"], o["past"])  # the state as it was: a pass can be made again
-    c.append(o["k"], o["v"], o["slots"], o["rows"])
+    # the state as it was: truncating leaves the exponents that the new rows raised, so the blocks
+    # that they joined begin again with the rows and exponents that they had
+    c.truncate(o["slots"], o["from"])
+    c.append(*o["begun"], o["slots"], o["older"], rotate=False)
+    k, v = (lh.Tensor.from_device(s["new_" + x]) for x in "kv")
+    c.append(k, v, o["slots"], o["rows"])
     k, v = c.read(o["slots"], o["from"], o["back"])
+    lh.sync()  # the results are there before another stream reads them
     return {"k": torch.as_tensor(k, device=DEV), "v": torch.as_tensor(v, device=DEV)}
 
 
-def _own_attention(o, lh):
-    return torch.as_tensor(o["cache"].attention(o["q"], o["slots"], o["rows"]), device=DEV)
+def _own_attention(s, o, lh):
+    out = o["cache"].attention(lh.Tensor.from_device(s["q"]), o["slots"], o["rows"])
+    lh.sync()
+    return torch.as_tensor(out, device=DEV)
 
 
-def _own_verify(o, lh):
-    accepted, tokens = lh.verify_drafts(o["target"], o["ids"], o["counts"], o["accept"], o["draw"], draft=o["draft"])
+def _own_verify(s, o, lh):
+    target, draft = (None if s[x] is None else lh.Tensor.from_device(s[x]) for x in ("target", "draft"))
+    ids, accept, draw = (s[x].cpu().numpy() for x in ("ids", "accept", "draw"))
+    accepted, tokens = lh.verify_drafts(target, ids, o["counts"], accept, draw, draft=draft)
     return {"accepted": accepted, "tokens": tokens}
 
 
