@@ -102,8 +102,10 @@ int llmrs_tensor_download(const llmrs_tensor* t, float* out, size_t count);
  * copy_device: a new f32 tensor from contiguous f32 values in device memory.
  * Waits for all work queued on that device, whatever its stream, and for the
  * copy, so `src` may be reused on return.  address: where an f32 tensor's values
- * are, valid until llmrs_tensor_free; work queued by this library may still be
- * writing there until llmrs_sync. */
+ * are, valid until llmrs_tensor_free.  Waits for all work queued by this library,
+ * so the values are there for every stream; what the library does with the tensor
+ * later (llmrs_add_assign on it, say) is for the caller to order: llmrs_sync after
+ * it, and a wait for the other library's work before it. */
 int llmrs_tensor_copy_device(const void* src, const size_t* dims, int ndim, llmrs_tensor** out);
 int llmrs_tensor_address(const llmrs_tensor* t, void** address);
 int llmrs_tensor_ndim(const llmrs_tensor* t);

@@ -177,6 +177,8 @@ int llmrs_tensor_address(const llmrs_tensor* t, void** address) {
   return guard([&] {
     require_f32(t, "address");
     LLMRS_REQUIRE(address, LLMRS_E_INVALID, "address is null");
+    // the library's stream is ordered with no other one, not even the null stream
+    LLMRS_HIP(hipStreamSynchronize(ctx().stream));
     *address = t->data;
   });
 }

@@ -316,8 +316,10 @@ class Tensor:
     @property
     def __cuda_array_interface__(self) -> dict:
         """An f32 tensor's values in place, for another library in this
-        process: while this object lives, and not before ``sync()`` where
-        work on them is still queued."""
+        process, while this object lives (llmrs_tensor_address).  Waits for
+        the library's queued work, so the values are there for every stream
+        (the protocol's version 3 without a ``stream``); work of the library
+        on this tensor after that is for the caller to order."""
         at, shape = C.c_void_p(), self.shape
         _check(lib().llmrs_tensor_address(self._h, C.byref(at)))
         return {"shape": shape, "typestr": "<f4", "data": (0 if 0 in shape else at.value, False), "version": 3}
