@@ -75,7 +75,8 @@ const char* llmrs_last_error(void);
 int llmrs_device(void);
 /* Backend::name (src/backend.rs:18). */
 const char* llmrs_name(void);
-/* Wait for all queued work (the reference's queue.finish()). */
+/* Wait for all queued work (the reference's queue.finish()); after tensors whose
+ * addresses were given out have been freed, for the whole device. */
 int llmrs_sync(void);
 /* Number of compute units of the current device (0 before init). */
 int llmrs_num_cus(void);
@@ -102,7 +103,9 @@ int llmrs_tensor_download(const llmrs_tensor* t, float* out, size_t count);
  * copy_device: a new f32 tensor from contiguous f32 values in device memory.
  * Waits for all work queued on that device, whatever its stream, and for the
  * copy, so `src` may be reused on return.  address: where an f32 tensor's values
- * are, valid until llmrs_tensor_free.  Waits for all work queued by this library,
+ * are, valid until llmrs_tensor_free (work of the other library that was queued
+ * before it may still read them: the memory is not used again before the device
+ * has been waited for).  Waits for all work queued by this library,
  * so the values are there for every stream; what the library does with the tensor
  * later (llmrs_add_assign on it, say) is for the caller to order: llmrs_sync after
  * it, and a wait for the other library's work before it. */

@@ -49,15 +49,22 @@ struct Error : std::runtime_error {
 
 // Size-bucketed caching allocator for operator outputs: the analogue of the
 // reference's OpenCL scratch pool (opencl.rs:36-90), without its per-token
-// reset - buffers return to their bucket when the tensor is freed.
+// reset - buffers return to their bucket when the tensor is freed.  Reuse follows
+// in the order of the library's stream; a block whose address another library was
+// given waits for the whole device first.
 class Allocator {
  public:
   void* alloc(size_t bytes);
   void release(void* p);
+  void hold(void* p);  // released once the device has been waited for
+  bool holds() const { return !held_.empty(); }
+  void device_waited();  // no work from before is left on the device
   void trim();  // hipFree every cached block
  private:
+  void* take(size_t size);
   std::multimap<size_t, void*> free_;
   std::map<void*, size_t> live_;
+  std::vector<void*> held_;
 };
 
 // Device scratch of llmrs_matmul_transposed_noalloc (noalloc.hip): a fixed
@@ -95,6 +102,23 @@ constexpr size_t kFetchBytes = (size_t)1 << 20;
 void fetch(void* dst, const void* src, size_t bytes, std::initializer_list<const int*> ints = {}, int* out = nullptr);
 
 Context& ctx();  // fails with LLMRS_E_NOINIT before llmrs_init
+// Makes the context's device the calling thread's for the scope (a caller may
+// have another one current).
+struct OnDevice {
+  int was = -1;
+  OnDevice() {
+    LLMRS_HIP(hipGetDevice(&was));
+    if (was != ctx().device) LLMRS_HIP(hipSetDevice(ctx().device));
+    else was = -1;
+  }
+  ~OnDevice() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+
+// Waits for the library's stream; where blocks are held, for all of its device,
+// and they are free.
+void wait_for_work();
 std::recursive_mutex& api_mutex();
 // The kernel `name`; fails (LLMRS_E_INVALID) when `block` exceeds the
 // threads per workgroup it was compiled for (its launch bounds).
@@ -221,6 +245,7 @@ struct llmrs_tensor {
   void* data = nullptr;       // f32 values, or codes of quantised tensors
   void* scales = nullptr;     // scales of quantised tensors (same allocation)
   size_t bytes = 0;
+  mutable bool lent = false;  // another library was given the address
   size_t numel() const {
     size_t n = 1;
     for (size_t d : dims) n *= d;

@@ -316,6 +316,25 @@ bool sgemm_faster(int wt, const std::string& epi, int m, int n, int k, int num_c
 }
 
 // ---- allocator -------------------------------------------------------------
+void wait_for_work() {
+  Context& c = ctx();
+  if (!c.alloc.holds()) {
+    LLMRS_HIP(hipStreamSynchronize(c.stream));
+    return;
+  }
+  OnDevice here;
+  LLMRS_HIP(hipDeviceSynchronize());
+  c.alloc.device_waited();
+}
+
+void* Allocator::take(size_t size) {
+  auto it = free_.find(size);
+  if (it == free_.end()) return nullptr;
+  void* p = it->second;
+  free_.erase(it);
+  return p;
+}
+
 void* Allocator::alloc(size_t bytes) {
   size_t sz = align_up(bytes ? bytes : 1, 256);
   if (sz > (1u << 20)) {  // round large requests to 1/8 octave to improve reuse
@@ -324,15 +343,12 @@ void* Allocator::alloc(size_t bytes) {
     size_t step = std::max<size_t>(p / 8, 256);
     sz = align_up(sz, step);
   }
-  auto it = free_.find(sz);
-  void* ptr = nullptr;
-  if (it != free_.end()) {
-    ptr = it->second;
-    free_.erase(it);
-  } else {
+  void* ptr = take(sz);
+  if (!ptr) {
     hipError_t e = hipMalloc(&ptr, sz);
     if (e != hipSuccess) {
       (void)hipGetLastError();
+      if (holds()) wait_for_work();
       trim();
       e = hipMalloc(&ptr, sz);
     }
@@ -351,6 +367,15 @@ void Allocator::release(void* p) {
   if (it == live_.end()) return;
   free_.emplace(it->second, p);
   live_.erase(it);
+}
+
+void Allocator::hold(void* p) {
+  if (live_.count(p)) held_.push_back(p);
+}
+
+void Allocator::device_waited() {
+  for (void* p : held_) release(p);
+  held_.clear();
 }
 
 void Allocator::trim() {
@@ -504,7 +529,10 @@ int llmrs_init(int device_ordinal, const char* hsaco_dir) {
 int llmrs_shutdown(void) {
   return guard([&] {
     if (!g_ctx) return;
-    (void)hipStreamSynchronize(g_ctx->stream);
+    try {
+      wait_for_work();
+    } catch (const Error&) {  // what is left ends all the same
+    }
     g_ctx->alloc.release(g_ctx->verify_tickets);
     g_ctx->alloc.trim();
     for (hipModule_t m : g_ctx->modules) (void)hipModuleUnload(m);
@@ -519,7 +547,7 @@ int llmrs_device(void) { return LLMRS_DEVICE_HIP; }
 const char* llmrs_name(void) { return "Hip"; }
 
 int llmrs_sync(void) {
-  return guard([&] { LLMRS_HIP(hipStreamSynchronize(ctx().stream)); });
+  return guard([&] { wait_for_work(); });
 }
 
 int llmrs_num_cus(void) { return g_ctx ? g_ctx->num_cus : 0; }

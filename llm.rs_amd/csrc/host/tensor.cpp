@@ -161,6 +161,7 @@ int llmrs_tensor_copy_device(const void* src, const size_t* dims, int ndim, llmr
       const hipError_t e = hipDeviceSynchronize();
       LLMRS_HIP(hipSetDevice(ctx().device));
       LLMRS_HIP(e);
+      if (at.device == ctx().device) ctx().alloc.device_waited();
     }
     std::unique_ptr<llmrs_tensor> t(alloc_f32(d));
     if (count) {
@@ -178,7 +179,8 @@ int llmrs_tensor_address(const llmrs_tensor* t, void** address) {
     require_f32(t, "address");
     LLMRS_REQUIRE(address, LLMRS_E_INVALID, "address is null");
     // the library's stream is ordered with no other one, not even the null stream
-    LLMRS_HIP(hipStreamSynchronize(ctx().stream));
+    wait_for_work();
+    t->lent = true;
     *address = t->data;
   });
 }
@@ -196,7 +198,8 @@ int llmrs_tensor_dtype(const llmrs_tensor* t) { return t ? t->dtype : LLMRS_E_IN
 int llmrs_tensor_free(llmrs_tensor* t) {
   return guard([&] {
     if (!t) return;
-    if (t->data) ctx().alloc.release(t->data);
+    if (t->lent) ctx().alloc.hold(t->data);  // the other library may have queued work that reads it
+    else if (t->data) ctx().alloc.release(t->data);
     delete t;
   });
 }

@@ -47,18 +47,4 @@ class LaunchWords {
   Scratch mem_;
 };
 
-// Makes the context's device the calling thread's for the scope (a caller may
-// have another one current).
-struct OnDevice {
-  int was = -1;
-  OnDevice() {
-    LLMRS_HIP(hipGetDevice(&was));
-    if (was != ctx().device) LLMRS_HIP(hipSetDevice(ctx().device));
-    else was = -1;
-  }
-  ~OnDevice() {
-    if (was >= 0) (void)hipSetDevice(was);
-  }
-};
-
 }  // namespace llmrs

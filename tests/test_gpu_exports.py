@@ -59,3 +59,49 @@ for stream in (torch.cuda.default_stream(), side):
             copies = [x.clone() for x in views]
             assert torch.equal(copies[0].cpu(), k) and torch.equal(copies[1].cpu(), v)
 """)
+
+
+def test_memory_outlives_what_still_reads_it():
+    """A view is dropped while work that reads it waits behind other work of its
+    stream; calls that follow do not write there."""
+    run("""
+side = torch.cuda.Stream()
+a = torch.zeros(1 << 26, device="cuda")
+torch.cuda.synchronize()
+for i in (0, 1, 0):
+    view = torch.as_tensor(cache.attention(q[i], [0], [rows]), device="cuda")
+    with torch.cuda.stream(side):
+        for _ in range(40):      # about 4 ms
+            a += 1
+        got = view.clone()
+    del view
+    for _ in range(4):
+        cache.attention(q[1 - i], [0], [rows])
+    side.synchronize()
+    assert torch.equal(got.cpu(), want[i])
+""")
+
+
+def test_memory_of_dropped_views_is_used_again():
+    """Not for the next tensor, but once the device has been waited for."""
+    run("""
+def address(t):
+    return t.__cuda_array_interface__["data"][0]
+seen, last = set(), None
+for _ in range(30):
+    t = cache.attention(q[0], [0], [rows])
+    assert address(t) != last
+    last = address(t)
+    seen.add(last)
+    del t
+assert len(seen) <= 4, len(seen)
+# (the first round's tensors are free before the second round's: it asks for more)
+for wait, n in ((hip.sync, 6), (lambda: hip.Tensor.from_device(torch.zeros(1, device="cuda")), 16)):
+    t = cache.attention(q[0], [0], [rows])
+    last = address(t)
+    del t
+    wait()
+    kept = [cache.attention(q[0], [0], [rows]) for _ in range(n)]
+    assert last in [address(t) for t in kept]
+    del kept
+""")
