@@ -152,6 +152,9 @@ __device__ __forceinline__ void slice_draw(const VerifyArgs& a, const Row& r, in
 __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const unsigned* part, double u) {
   const int lane = lane_id(), groups = a.groups;
   double x[kHeld];  // running sums of 64 slices each
+  // the slices that hold anything: the running sums are formed as trees, so one may
+  // rise by a last place past a slice that does not
+  unsigned long long some[kHeld];
   auto hold = [&](int g0) {
 #pragma unroll
     for (int c = 0; c < kHeld; ++c) {
@@ -159,8 +162,10 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const uns
       x[c] = g < groups ? __builtin_bit_cast(double, dev_ld8(part, 8 * g)) : 0.0;
     }
 #pragma unroll
-    for (int c = 0; c < kHeld; ++c)
+    for (int c = 0; c < kHeld; ++c) {
+      some[c] = __ballot(x[c] > 0.0);
       if (g0 + LLMRS_WAVE * c < groups) x[c] = scan(x[c]);
+    }
   };
   constexpr int HELD = LLMRS_WAVE * kHeld;
   double total = 0.0;
@@ -196,15 +201,14 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const uns
 #pragma unroll
     for (int c = 0; c < kHeld; ++c) {
       if (g0 + LLMRS_WAVE * c >= groups) break;
-      const unsigned long long over = __ballot(base + x[c] > tau);
+      const unsigned long long over = __ballot(base + x[c] > tau) & some[c];
       const double before = dpp64<0x138, 0xF>(x[c]);
-      const unsigned long long holds = __ballot(x[c] > before);
       if (slice < 0 && over) {
         const int l = __builtin_ctzll(over);
         slice = g0 + LLMRS_WAVE * c + l;
         from = base + lane64(before, l);
       }
-      if (slice < 0 && holds) top = g0 + LLMRS_WAVE * c + last_of(holds);
+      if (slice < 0 && some[c]) top = g0 + LLMRS_WAVE * c + last_of(some[c]);
       base += lane64(x[c], 63);
     }
   }

@@ -3,6 +3,7 @@ GPU, against numpy in 64 bits (paged_ref.py).  Codes are compared exactly;
 the attention within the bound that the reference derives."""
 from __future__ import annotations
 
+import math
 import os
 import subprocess
 import sys
@@ -521,6 +522,50 @@ def test_verify_borders(hip):
             for d in (q, p, None):
                 check_verify(hip, np.stack([p, q]), ids, [1], np.float32([accept]), np.float32([draw]),
                              None if d is None else d[None])
+
+
+def lanes_scanned(v):
+    """Running sums of 64 numbers in 64 bits, in the order in which a wave forms them:
+    by steps of 1, 2, 4 and 8 within each 16, then the 16s' totals."""
+    v = np.asarray(v, np.float64).reshape(4, 16)
+    for step in (1, 2, 4, 8):
+        v = v + np.concatenate((np.zeros((4, step)), v[:, :-step]), 1)
+    v = v + np.array([0.0, v[0, 15], 0.0, v[2, 15]])[:, None]
+    return (v + np.array([0.0, 0.0, v[1, 15], v[1, 15]])[:, None]).reshape(64)
+
+
+def test_verify_draws_nothing_from_empty_slices(hip):
+    """Rows with an id in few of the sums' slices, as top-k leaves them.  The running sum
+    over the slices is formed as a tree, so behind an empty one it may be a last place
+    larger than before it; a draw that meets the sum there takes an id that has something.
+    64 numbers of one sign in whatever order are off by up to 63 roundings of their sum, on
+    either side of the comparison: the ids whose exact running sum reaches half of the total
+    less that, while the one before them does not exceed half and that."""
+    rng = np.random.default_rng(17)
+    rows, at = [], []
+    while len(rows) < 12:
+        n = int(rng.integers(3, 12))
+        slices = np.sort(rng.choice(30, n, replace=False))
+        w = np.zeros(32, np.float32)
+        w[slices] = (10.0 ** rng.uniform(-16, 0, n)).astype(np.float32)
+        sums = np.concatenate((w, w)).astype(np.float64)  # both halves alike: half of the total ends the first
+        running = lanes_scanned(sums)
+        if sums[np.nonzero(running > 0.5 * running[63])[0][0]] > 0:
+            continue
+        row, ids = np.zeros(64 * 512, np.float32), rng.integers(0, 512, 64) + 512 * np.arange(64)
+        row[ids] = sums
+        rows.append(row)
+        exact = [math.fsum(sums[:i]) for i in range(65)]
+        room = 2 * 64 * 2.0 ** -53 * exact[64]
+        at.append({int(ids[i]) for i in range(64) if sums[i] > 0 and exact[i + 1] >= exact[64] / 2 - room and exact[i] <= exact[64] / 2 + room})
+        assert {int(ids[slices[-1]]), int(ids[32 + slices[0]])} <= at[-1]
+    target = np.stack(rows)
+    # after other slices as well, past the sums that a wave holds at once
+    for before in (0, 512 * 512, 512 * 512 * 3):
+        wide = np.concatenate((np.zeros((len(rows), before), np.float32), target), 1)
+        _, tokens = hip.verify_drafts(hip.Tensor.from_numpy(wide), [], [0] * len(rows), [], [0.5] * len(rows))
+        for i, ids in enumerate(at):
+            assert tokens[i, 0] - before in ids, (i, before, tokens[i, 0], ids)
 
 
 def test_verify_odd_rows(hip):
