@@ -413,8 +413,9 @@ int llmrs_batch_profile_step(llmrs_batch* b, char* names, float* ms, double* wor
  * as 127 * 2^121.
  *
  * The page table and the lengths are checked and kept on the host: a call with
- * an unknown slot, a slot named twice, a page in use, or positions without a
- * page is refused and changes nothing.  Device memory is taken by the first
+ * an unknown slot, a slot named twice, a page in use, positions without a page,
+ * or more work than a launch can have (2^32 threads) is refused and changes
+ * nothing.  Device memory is taken by the first
  * append.  Calls are queued on the library's stream and do not wait. */
 typedef struct llmrs_paged llmrs_paged;
 typedef struct {
@@ -458,6 +459,13 @@ int llmrs_paged_read(llmrs_paged* p, const int32_t* slots, const int32_t* starts
  * sequence's last bits may change with its company. */
 int llmrs_paged_attention(llmrs_paged* p, const llmrs_tensor* q, const int32_t* slots, const int32_t* counts, size_t n,
                           llmrs_tensor** out);
+
+/* Test probe: the columns (query rows x heads of a KV head's group) that a
+ * workgroup of llmrs_paged_attention takes for each sequence of a call, 16 or 64,
+ * and in how many splits it takes the sequence's positions (0 and 0 without rows).
+ * group: query heads per KV head; lengths: with the new rows.  Needs no device. */
+int llmrs_probe_paged_plan(int n_kv_heads, int head_dim, int group, const int32_t* lengths, const int32_t* counts, size_t n,
+                           int num_cus, int32_t* columns, int32_t* splits);
 
 /* ---- verification of drafted tokens (no reference counterpart) -------------
  * For n sequences with counts[i] (0 to 64) drafted tokens each: `target` f32

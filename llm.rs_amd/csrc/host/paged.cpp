@@ -114,18 +114,35 @@ void require_rows(const llmrs_tensor* t, size_t rows, size_t width, const std::s
                 what + ": must be [" + std::to_string(rows) + ", " + std::to_string(width) + "]");
 }
 
-// What the kernels know of the parts; items[i]: work items of part i.
-std::vector<int> seq_words(const std::vector<Part>& parts, const std::vector<int>& items, int* total) {
+// The work items of a launch, each part's; refused where `threads` of them for each item
+// are more than a launch can have in one dimension (2^32 less one).
+struct Items {
+  std::vector<int> of;
+  int total = 0;
+};
+template <class F>
+Items count_items(const std::vector<Part>& parts, size_t threads, const char* what, F&& items) {
+  Items n;
+  size_t at = 0;
+  for (const Part& s : parts) {
+    at += items(s);
+    LLMRS_REQUIRE(at * threads < ((size_t)1 << 32), LLMRS_E_INVALID, std::string(what) + ": too much work for one call");
+    n.of.push_back((int)items(s));
+  }
+  n.total = (int)at;
+  return n;
+}
+
+// What the kernels know of the parts.
+std::vector<int> seq_words(const std::vector<Part>& parts, const Items& items) {
   std::vector<int> w;
   w.reserve(kPagedPerSeq * parts.size());
-  long at = 0;
-  for (int n : items) {
-    w.push_back((int)at);
+  int at = 0;
+  for (int n : items.of) {
+    w.push_back(at);
     at += n;
   }
-  LLMRS_REQUIRE(at <= (1 << 30), LLMRS_E_INVALID, "paged cache: too much work for one call");
   for (const Part& s : parts) w.insert(w.end(), {s.slot, s.row0, s.rows, s.pos});
-  *total = (int)at;
   return w;
 }
 
@@ -144,11 +161,14 @@ struct TensorFree {
 };
 typedef std::unique_ptr<llmrs_tensor, TensorFree> Rows;
 
-// One launch over the blocks that the parts' rows touch.
-void launch_rows(const llmrs_paged* p, const std::string& kernel, const std::vector<Part>& parts, float* k, float* v,
-                 bool rotate) {
-  std::vector<int> items;
-  for (const Part& s : parts) items.push_back((s.pos % kPagedBlock + s.rows + kPagedBlock - 1) / kPagedBlock);
+// The blocks that the parts' rows touch.
+Items row_items(const llmrs_paged* p, const std::vector<Part>& parts, const char* what) {
+  return count_items(parts, 2 * (size_t)p->cfg.head_dim, what,
+                     [](const Part& s) { return (size_t)(s.pos % kPagedBlock + s.rows + kPagedBlock - 1) / kPagedBlock; });
+}
+// One launch over them.
+void launch_rows(const llmrs_paged* p, const std::string& kernel, const std::vector<Part>& parts, const Items& items,
+                 float* k, float* v, bool rotate) {
   PagedRowsArgs a;
   a.pool = p->pool();
   a.rows[0] = k;
@@ -156,7 +176,8 @@ void launch_rows(const llmrs_paged* p, const std::string& kernel, const std::vec
   a.rope_cos = rotate ? p->cos() : nullptr;
   a.rope_sin = rotate ? p->sin() : nullptr;
   a.seqs.n = (int)parts.size();
-  const LaunchWords words(seq_words(parts, items, &a.seqs.items), a.seqs.w);
+  a.seqs.items = items.total;
+  const LaunchWords words(seq_words(parts, items), a.seqs.w);
   a.seqs.ext = words.ext();
   launch(kernel + hd_tag(p), dim3((unsigned)a.seqs.items, (unsigned)p->cfg.n_kv_heads, 2),
          dim3((unsigned)(2 * p->cfg.head_dim)), 0, ctx().stream, a);
@@ -206,9 +227,44 @@ int split_units(const std::vector<Part>& parts, long heads, int n_rep, int hd, c
   return std::min(per, most);
 }
 
-void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, const std::vector<Part>& parts,
-                      AttnKind kind) {
-  const int nkv = p->cfg.n_kv_heads, hd = p->cfg.head_dim, cols = kind.cols;
+// One launch of the attention: its sequences, kernel and splits.
+struct AttnPlan {
+  explicit AttnPlan(const AttnKind& k) : kind(k) {}
+  AttnKind kind;
+  std::vector<Part> parts;
+  int chunk = 0;  // positions of a split, at most
+  bool split = false;
+  Items items;
+  int splits(const Part& s) const { return (s.pos + chunk - 1) / chunk; }
+};
+
+// The launches of a call.  The kernel of 64 columns reads a cache a quarter as often, but
+// needs columns for every CU's waves; sequences that do not fill one of its workgroups
+// stay with the kernel of 16.
+std::vector<AttnPlan> plan_attention(const std::vector<Part>& parts, int nkv, int n_rep, int hd, int cus) {
+  AttnPlan few(kFew), many(kMany);
+  long columns = 0;
+  for (const Part& s : parts) {
+    const bool fills = (long)s.rows * n_rep >= kMany.cols;
+    (fills ? many : few).parts.push_back(s);
+    if (fills) columns += (long)s.rows * n_rep * nkv;
+  }
+  if (columns < kManyColumns * cus) few.parts = parts, many.parts.clear();
+  std::vector<AttnPlan> plans;
+  for (AttnPlan* p : {&few, &many}) {
+    if (p->parts.empty()) continue;
+    p->chunk = split_units(p->parts, nkv, n_rep, hd, p->kind, cus) * p->kind.unit;
+    p->items = count_items(p->parts, 256 * (size_t)nkv, "paged_attention", [&](const Part& s) {
+      return (size_t)p->splits(s) * (((size_t)s.rows * (size_t)n_rep + (size_t)p->kind.cols - 1) / (size_t)p->kind.cols);
+    });
+    for (const Part& s : p->parts) p->split = p->split || p->splits(s) > 1;
+    plans.push_back(std::move(*p));
+  }
+  return plans;
+}
+
+void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, const AttnPlan& plan) {
+  const int nkv = p->cfg.n_kv_heads, hd = p->cfg.head_dim;
   PagedAttnArgs a;
   a.pool = p->pool();
   a.q = (const float*)q->data;
@@ -217,27 +273,18 @@ void launch_attention(llmrs_paged* p, const llmrs_tensor* q, llmrs_tensor* out, 
   a.rope_sin = p->sin();
   a.nq = (int)(q->dims[1] / (size_t)hd);
   a.scale = 1.0f / std::sqrt((float)hd);
-  const int n_rep = a.nq / nkv, unit = kind.unit;
-  const int per = split_units(parts, nkv, n_rep, hd, kind, ctx().num_cus);
-  a.chunk = per * unit;
-  std::vector<int> items;
-  bool split = false;
-  for (const Part& s : parts) {
-    const int n = (s.pos + a.chunk - 1) / a.chunk;
-    items.push_back(n * ((s.rows * n_rep + cols - 1) / cols));
-    split = split || n > 1;
-  }
-  a.seqs.n = (int)parts.size();
-  const LaunchWords words(seq_words(parts, items, &a.seqs.items), a.seqs.w);
+  a.chunk = plan.chunk;
+  a.seqs.n = (int)plan.parts.size();
+  a.seqs.items = plan.items.total;
+  const LaunchWords words(seq_words(plan.parts, plan.items), a.seqs.w);
   a.seqs.ext = words.ext();
-  LLMRS_REQUIRE((long)a.seqs.items * nkv < (1L << 31), LLMRS_E_INVALID, "paged_attention: too much work for one call");
-  const size_t columns = split ? (size_t)a.seqs.items * nkv * cols : 0;
+  const size_t groups = (size_t)plan.items.total * (size_t)nkv;
+  const size_t columns = plan.split ? groups * (size_t)plan.kind.cols : 0;
   Scratch part(columns * 4 * (size_t)(hd + 2));
   a.part_o = (float*)part.p;
-  a.part_ml = a.part_o ? a.part_o + columns * hd : nullptr;
-  a.tickets = split ? p->zero_tickets((size_t)a.seqs.items * nkv) : nullptr;
-  const dim3 grid((unsigned)(a.seqs.items * nkv));
-  launch(std::string("paged_attn_") + kind.name + hd_tag(p), grid, dim3(256), 0, ctx().stream, a);
+  a.part_ml = a.part_o ? a.part_o + columns * (size_t)hd : nullptr;
+  a.tickets = plan.split ? p->zero_tickets(groups) : nullptr;
+  launch(std::string("paged_attn_") + plan.kind.name + hd_tag(p), dim3((unsigned)groups), dim3(256), 0, ctx().stream, a);
 }
 
 }  // namespace
@@ -368,13 +415,14 @@ int llmrs_paged_append(llmrs_paged* p, const llmrs_tensor* k, const llmrs_tensor
       LLMRS_REQUIRE(end <= p->cfg.max_seq && end <= (long)p->mapped[(size_t)s.slot] * p->cfg.page_size, LLMRS_E_RANGE,
                     "paged_append: slot " + std::to_string(s.slot) + " has no page for position " + std::to_string(end - 1));
     }
+    const Items items = row_items(p, parts, "paged_append");
     require_rows(k, rows, width, "paged_append k");
     require_rows(v, rows, width, "paged_append v");
     if (parts.empty()) return;
     (void)ctx();
     OnDevice here;
     p->settle();
-    launch_rows(p, "paged_append", parts, (float*)k->data, (float*)v->data, rotate != 0);
+    launch_rows(p, "paged_append", parts, items, (float*)k->data, (float*)v->data, rotate != 0);
     for (const Part& s : parts) p->length[(size_t)s.slot] += s.rows;
   });
 }
@@ -391,11 +439,12 @@ int llmrs_paged_read(llmrs_paged* p, const int32_t* slots, const int32_t* starts
                         " of " + std::to_string(p->length[(size_t)slots[s]]) + " in slot " + std::to_string(slots[s]));
       if (counts[s]) parts[i++].pos = starts[s];
     }
+    const Items items = row_items(p, parts, "paged_read");
     (void)ctx();
     OnDevice here;
     const size_t width = (size_t)p->cfg.n_kv_heads * (size_t)p->cfg.head_dim;
     Rows kr(new_rows(rows, width)), vr(new_rows(rows, width));
-    if (!parts.empty()) launch_rows(p, "paged_read", parts, (float*)kr->data, (float*)vr->data, false);
+    if (!parts.empty()) launch_rows(p, "paged_read", parts, items, (float*)kr->data, (float*)vr->data, false);
     *k = kr.release();
     *v = vr.release();
   });
@@ -416,24 +465,33 @@ int llmrs_paged_attention(llmrs_paged* p, const llmrs_tensor* q, const int32_t* 
     LLMRS_REQUIRE(q->dims.size() == 2 && q->dims[1] > 0 && q->dims[1] % group == 0 && q->dims[1] <= 65536, LLMRS_E_INVALID,
                   "paged_attention: q must be [rows, query heads * head_dim] with whole groups of query heads");
     require_rows(q, rows, q->dims[1], "paged_attention q");
-    (void)ctx();
     OnDevice here;
+    const std::vector<AttnPlan> plans =
+        plan_attention(parts, p->cfg.n_kv_heads, (int)(q->dims[1] / group), p->cfg.head_dim, ctx().num_cus);
     Rows o(new_rows(rows, q->dims[1]));
-    // The kernel of 64 columns reads a cache a quarter as often, but needs columns for
-    // every CU's waves; sequences that do not fill one of its workgroups stay with the
-    // kernel of 16.
-    const long n_rep = (long)(q->dims[1] / group);
-    std::vector<Part> few, many;
-    long columns = 0;
-    for (const Part& s : parts) {
-      const bool fills = s.rows * n_rep >= kMany.cols;
-      (fills ? many : few).push_back(s);
-      if (fills) columns += s.rows * n_rep * p->cfg.n_kv_heads;
-    }
-    if (columns < kManyColumns * ctx().num_cus) few = parts, many.clear();
-    if (!few.empty()) launch_attention(p, q, o.get(), few, kFew);
-    if (!many.empty()) launch_attention(p, q, o.get(), many, kMany);
+    for (const AttnPlan& plan : plans) launch_attention(p, q, o.get(), plan);
     *out = o.release();
+  });
+}
+
+int llmrs_probe_paged_plan(int n_kv_heads, int head_dim, int group, const int32_t* lengths, const int32_t* counts, size_t n,
+                           int num_cus, int32_t* columns, int32_t* splits) {
+  return guard([&] {
+    LLMRS_REQUIRE(lengths && counts && columns && splits, LLMRS_E_INVALID, "probe_paged_plan: null argument");
+    LLMRS_REQUIRE(n_kv_heads >= 1 && n_kv_heads <= 256 && (head_dim == 64 || head_dim == 128) && group >= 1 && group <= 1024 &&
+                      num_cus > 0 && n <= 65536, LLMRS_E_INVALID, "probe_paged_plan: bad argument");
+    std::vector<Part> parts;
+    for (size_t i = 0; i < n; ++i) {
+      LLMRS_REQUIRE(counts[i] >= 0 && counts[i] <= lengths[i] && lengths[i] <= (1 << 20), LLMRS_E_RANGE,
+                    "probe_paged_plan: bad length");
+      columns[i] = splits[i] = 0;
+      if (counts[i]) parts.push_back({(int)i, 0, counts[i], lengths[i]});
+    }
+    for (const AttnPlan& plan : plan_attention(parts, n_kv_heads, group, head_dim, num_cus))
+      for (const Part& s : plan.parts) {
+        columns[s.slot] = plan.kind.cols;
+        splits[s.slot] = plan.splits(s);
+      }
   });
 }
 

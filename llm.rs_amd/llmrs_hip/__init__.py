@@ -141,6 +141,8 @@ _SIGS = {
                                    C.POINTER(C.c_void_p)]),
     "llmrs_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                         C.POINTER(C.c_void_p)]),
+    "llmrs_probe_paged_plan": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p,
+                                         C.c_void_p]),
     "llmrs_verify_drafts": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                       C.c_void_p, C.c_void_p, C.c_size_t]),
     "llmrs_synth_q4": (C.c_int, [C.c_uint64, C.c_uint64, C.c_size_t, C.c_size_t, C.c_float, C.c_float, C.c_void_p, C.c_void_p, C.c_int]),
@@ -860,6 +862,16 @@ class HipPagedCache:
         out = C.c_void_p()
         _check(lib().llmrs_paged_attention(self._h, q.handle, _ref(slots), _ref(counts), slots.size, C.byref(out)))
         return Tensor(out, q.shape)
+
+
+def probe_paged_plan(n_kv_heads: int, head_dim: int, group: int, lengths, counts, cus: int = 256) -> tuple[list[int], list[int]]:
+    """Columns per workgroup and splits of each sequence of an attention call
+    (llmrs_probe_paged_plan); needs no device."""
+    lengths, counts = _pair(lengths, counts, "probe_paged_plan")
+    columns, splits = np.empty(counts.size, np.int32), np.empty(counts.size, np.int32)
+    _check(lib().llmrs_probe_paged_plan(n_kv_heads, head_dim, group, _ref(lengths), _ref(counts), counts.size, cus,
+                                        _ref(columns), _ref(splits)))
+    return columns.tolist(), splits.tolist()
 
 
 def verify_drafts(target: Tensor, ids, counts, accept, draw, draft: Tensor | None = None) -> tuple[np.ndarray, np.ndarray]:

@@ -154,3 +154,22 @@ def test_from_device_takes_device_memory_only():
             self.__cuda_array_interface__ = {"shape": (2, 3), "typestr": "<f4", "data": (0, False), "version": 3} | kw
     refused(lh.E_DTYPE, lh.Tensor.from_device, Fake(typestr="<f2"))
     refused(lh.E_INVALID, lh.Tensor.from_device, Fake(strides=(4, 8)))
+
+
+def test_more_work_than_a_launch_has_threads():
+    """2^32 threads in one dimension are refused, before any tensor is looked at; one
+    sequence less is not."""
+    c, no = cache(head_dim=128, page_size=4096, n_pages=2 * 65536, max_seqs=65536, max_seq=8192), NoTensor()
+    for slot in range(65536):
+        c.map(slot, [2 * slot, 2 * slot + 1])
+    slots, rows = np.arange(65536, dtype=np.int32), np.full(65536, 8192, np.int32)  # 2^24 blocks of 256 threads
+    assert "too much work" in refused(lh.E_INVALID, c.append, no, no, slots, rows)
+    assert "null tensor" in refused(lh.E_INVALID, c.append, no, no, slots[:-1], rows[:-1])
+    assert c.length(0) == c.length(65535) == 0
+    # 2^24 workgroups of attention
+    ones = np.ones(65536, np.int32)
+    assert "too much work" in refused(lh.E_INVALID, lh.probe_paged_plan, 256, 64, 1, ones, ones)
+    assert lh.probe_paged_plan(256, 64, 1, ones[:-1], ones[:-1]) == ([16] * 65535, [1] * 65535)
+    # the launch of the second kernel too is looked at before the first is queued
+    lengths, counts = np.append(ones, 1 << 20), np.append(ones, 1 << 20)
+    assert "too much work" in refused(lh.E_INVALID, lh.probe_paged_plan, 256, 64, 64, lengths[1:], counts[1:])
