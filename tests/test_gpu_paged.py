@@ -349,6 +349,12 @@ def test_attention_many_columns(hip, nq, nkv, hd, page, lens, counts):
     check_sample(b, nq, slots, counts)
 
 
+def test_tested_calls_take_their_kernels(hip):
+    """On this device's CUs, whose number the plan goes by."""
+    from test_paged import check_tested_plans
+    check_tested_plans(hip.num_cus())
+
+
 def test_attention_many_columns_scores_of_any_size(hip):
     """As for few columns: zeros, peaked softmaxes, one sign past f32's steps."""
     b = Both(hip, 8, 128, max_seq=1024, rope=None)

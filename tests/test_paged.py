@@ -173,3 +173,37 @@ def test_more_work_than_a_launch_has_threads():
     # the launch of the second kernel too is looked at before the first is queued
     lengths, counts = np.append(ones, 1 << 20), np.append(ones, 1 << 20)
     assert "too much work" in refused(lh.E_INVALID, lh.probe_paged_plan, 256, 64, 64, lengths[1:], counts[1:])
+
+
+def test_plan_covers_every_position():
+    """Splits of at most 64, none longer than the sequence, and rows without any."""
+    for kv, hd, group in ((1, 64, 1), (8, 128, 4), (2, 64, 20), (8, 64, 8), (16, 128, 1)):
+        for lengths in ([1], [1, 255, 256, 257], [1 << 20], [4000] * 300, [9000] + [40] * 70, list(range(1, 2000, 37))):
+            for rows in (0, 1, 5, 64, 700):
+                counts = [min(rows, n) for n in lengths]
+                columns, splits = lh.probe_paged_plan(kv, hd, group, lengths, counts)
+                for n, r, c, s in zip(lengths, counts, columns, splits):
+                    assert (c, s) == (0, 0) if r == 0 else c in (16, 64) and 1 <= s <= min(64, -(-n // (256 if c == 16 else 64)))
+    refused(lh.E_RANGE, lh.probe_paged_plan, 1, 64, 1, [3], [4])
+    refused(lh.E_INVALID, lh.probe_paged_plan, 0, 64, 1, [3], [3])
+
+
+def test_plans_of_the_tested_calls():
+    """The calls by which test_gpu_paged.py tests the kernel of 64 columns and the
+    joining of splits come to it, on 256 CUs."""
+    check_tested_plans(256)
+
+
+def check_tested_plans(cus):
+    from test_gpu_paged import MANY
+    for nq, kv, hd, _, lens, counts in MANY:
+        columns, _ = lh.probe_paged_plan(kv, hd, nq // kv, lens, counts, cus)
+        assert columns == [0 if not r else 64 if r * nq // kv >= 64 else 16 for r in counts]
+    assert lh.probe_paged_plan(8, 128, 4, [850], [800], cus)[0] == [64]
+    assert lh.probe_paged_plan(8, 128, 4, [850, 40], [800, 1], cus)[0] == [64, 16]
+    for lens, counts, columns in (([9000] + [40] * 70, [1] * 71, 16), ([9000, 300, 300], [16, 300, 300], 64)):
+        c, s = lh.probe_paged_plan(8, 64, 8, lens, counts, cus)
+        assert set(c) == {columns} and s[0] > 1 and set(s[1:]) == {1}
+    for kv, length, rows in ((2, 5000, 1), (2, 5000, 6), (1, 1300, 2), (1, 1300, 600)):
+        assert lh.probe_paged_plan(kv, 128, 4, [length], [rows], cus)[1][0] > 1
+    assert lh.probe_paged_plan(8, 128, 4, [999, 500, 1, 64], [3, 2, 1, 1], cus)[1][0] > 1
