@@ -772,6 +772,17 @@ def _vec(a, dtype) -> np.ndarray:
     return out
 
 
+def _draws(a) -> np.ndarray:
+    """Uniform numbers in [0, 1) as f32: those of wider types that are nearest to 1
+    stay below it."""
+    x = _vec(a, _F32)
+    if x is not a:
+        up = (x == 1) & (np.asarray(a).reshape(-1) < 1)
+        if up.any():
+            x = np.where(up, np.nextafter(_F32.type(1), _F32.type(0)), x)
+    return x
+
+
 _I32, _F32 = np.dtype(np.int32), np.dtype(np.float32)
 
 
@@ -878,7 +889,7 @@ def verify_drafts(target: Tensor, ids, counts, accept, draw, draft: Tensor | Non
     """Drafted tokens against the target's probabilities, from given uniform
     numbers (llmrs_verify_drafts): accepted drafts per sequence, and their ids
     followed by the next token's, -1 past it."""
-    ids, counts, accept, draw = _vec(ids, _I32), _vec(counts, _I32), _vec(accept, _F32), _vec(draw, _F32)
+    ids, counts, accept, draw = _vec(ids, _I32), _vec(counts, _I32), _vec(accept, _F32), _draws(draw)
     each = counts.tolist()
     if min(each, default=0) < 0 or ids.size != sum(each) or accept.size != ids.size or draw.size != counts.size:
         raise LlmrsError(E_INVALID, "verify_drafts: one id and one number per draft, one draw per sequence")

@@ -586,6 +586,19 @@ def test_verify_odd_rows(hip):
         assert accepted[0] == 0 and tokens[0].tolist() == [4000, -1]
 
 
+def test_verify_draws_of_64_bits(hip):
+    """A number below 1 that f32 has no nearer neighbour for than 1 is a draw all the same."""
+    p = hip.Tensor.from_numpy(np.full((2, 6), 1 / 6, np.float32))
+    top = 1.0 - 2.0 ** -53
+    for draw in ([top, 0.5], np.array([top, 0.5]), np.array([[top], [0.5]])):
+        accepted, tokens = hip.verify_drafts(p, [], [0, 0], [], draw)
+        assert accepted.tolist() == [0, 0] and tokens[:, 0].tolist() == [5, 3]
+    for draw in ([1.0, 0.5], np.array([1.0, 0.5]), np.float32([1.0, 0.5]), [np.nan, 0.5], [1.0 + 2.0 ** -30, 0.5]):
+        with pytest.raises(hip.LlmrsError) as e:
+            hip.verify_drafts(p, [], [0, 0], [], draw)
+        assert e.value.code == hip.E_INVALID
+
+
 def test_verify_refusals(hip):
     T = hip.Tensor.from_numpy
     p, q = np.full((3, 5), 0.2, np.float32), np.full((2, 5), 0.2, np.float32)

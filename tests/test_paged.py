@@ -207,3 +207,11 @@ def check_tested_plans(cus):
     for kv, length, rows in ((2, 5000, 1), (2, 5000, 6), (1, 1300, 2), (1, 1300, 600)):
         assert lh.probe_paged_plan(kv, 128, 4, [length], [rows], cus)[1][0] > 1
     assert lh.probe_paged_plan(8, 128, 4, [999, 500, 1, 64], [3, 2, 1, 1], cus)[1][0] > 1
+
+
+def test_draws_stay_below_one():
+    top = np.float32(1.0 - 2.0 ** -24)
+    x = lh._draws([1.0 - 2.0 ** -53, 1.0, 0.25, 1.0 - 2.0 ** -26])
+    assert x.dtype == np.float32 and x.tolist() == [top, 1.0, 0.25, top]
+    same = np.float32([1.0, 0.5])
+    assert lh._draws(same) is same
