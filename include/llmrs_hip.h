@@ -408,15 +408,20 @@ int llmrs_batch_profile_step(llmrs_batch* b, char* names, float* ms, double* wor
  * positions, KV head and K or V: value = code * 2^e, e the smallest exponent in
  * [-100, 121] for which the largest magnitude of the block's rows is at most
  * 127 * 2^e.  Rows that join a block may raise e; the codes already there are
- * rounded to the new step (half to even).  Truncating leaves e as it is; a block
- * that is begun again starts afresh.  NaN is stored as zero, larger magnitudes
- * as 127 * 2^121.
+ * rounded to the new step (half to even).  Truncating leaves e and the codes as
+ * they are; a block that is begun again starts afresh.  So rows that are taken
+ * back (drafts that were refused) may leave the older rows of their block rounded
+ * to a coarser step, which later rows of that block get too: decoding with drafts
+ * is decoding without them to within the steps of the cache, not bit for bit.  NaN
+ * (also what rotation makes of an infinity: infinity times zero) is stored as
+ * zero, larger magnitudes as 127 * 2^121.
  *
  * The page table and the lengths are checked and kept on the host: a call with
  * an unknown slot, a slot named twice, a page in use, positions without a page,
  * or more work than a launch can have (2^32 threads) is refused and changes
- * nothing.  Device memory is taken by the first
- * append.  Calls are queued on the library's stream and do not wait. */
+ * nothing.  Device memory is taken by the first append, which waits for its copies
+ * of the tables; all other calls are queued on the library's stream and do not
+ * wait. */
 typedef struct llmrs_paged llmrs_paged;
 typedef struct {
   int32_t n_kv_heads;  /* 1 to 256 */
@@ -454,7 +459,8 @@ int llmrs_paged_read(llmrs_paged* p, const int32_t* slots, const int32_t* starts
  * same shape.  Row t of a sequence of length L and count c sits at position p =
  * L - c + t: softmax over the positions up to p of (rotated q . K) / sqrt(head_dim),
  * times V.  Query head h reads KV head h / (query heads / KV heads).  A q row
- * with a NaN or an infinity gives NaN in that head alone.  The same call gives the
+ * with a NaN or an infinity gives NaN in that head alone; scores past 2e38 do not
+ * fit f32, and their head is not what the formula says.  The same call gives the
  * same bits; how long sequences are split follows from all of a call's, so a
  * sequence's last bits may change with its company. */
 int llmrs_paged_attention(llmrs_paged* p, const llmrs_tensor* q, const int32_t* slots, const int32_t* counts, size_t n,
@@ -476,9 +482,12 @@ int llmrs_probe_paged_plan(int n_kv_heads, int head_dim, int group, const int32_
  * [0, 1) per sequence.  Draft x is accepted while accept * draft[x] <
  * target[x] (exactly).  The first refused one is replaced by a draw from
  * max(target - draft, 0); after the last accepted one a token is drawn from the
- * target's last row.  A draw takes the smallest id whose running sum in 64 bits
- * exceeds draw * total; where nothing is left of the target, from the target as
- * it is.  NaN counts as zero; a row with nothing in it gives the last id.
+ * target's last row.  A draw takes the smallest id whose running sum exceeds draw *
+ * total, to within the roundings of the sums in 64 bits (a fixed order, so the same
+ * call draws the same id) and always one that has something; where nothing is left
+ * of the target, from the target as it is.  A comparison with NaN refuses the draft;
+ * a probability that is NaN, or whose draft's is, has nothing; a row with nothing in
+ * it gives the last id.
  * Writes per sequence the number of accepted drafts and, in a row of `width` >=
  * largest count + 1 ids, these, the drawn id and -1 for the rest.  Returns when
  * they are there. */

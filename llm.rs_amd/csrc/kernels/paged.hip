@@ -123,9 +123,10 @@ constexpr int block_threads(int hd) { return 2 * hd; }
 // Older codes are loaded and, where the new rows raise the exponent, rounded to the
 // new step.  K is rotated in 64 bits (the products of f32 values are exact there), so
 // a code does not depend on how a sum was rounded.
-// Bound by memory for prompts: 4 x 2048 rows of 8 heads x 128 in 18.0 us, 84 MB at 4.7
-// TB/s (a copy reaches 5.1); with the codes passed through LDS byte by byte it was about
-// 25.  A decode step of 64 sequences takes 5.1 us and one row 3.3, a chain of
+// Bound by memory for prompts: 4 x 2048 rows of 8 heads x 128 in 20.5 us (median of 125
+// launches; the fastest 18.7), 84 MB at 4.1 to 4.5 TB/s (a copy reaches 5.1); with the
+// codes passed through LDS byte by byte the fastest was about 25.  A decode step of 64
+// sequences takes 5.1 us and one row 3.3, a chain of
 // dependent accesses (words, page, exponent, codes); 64-bit work where no new row is made
 // it 6.8.
 template <int HD>
@@ -242,7 +243,8 @@ extern "C" __global__ __launch_bounds__(block_threads(64)) void paged_append_hd6
 extern "C" __global__ __launch_bounds__(block_threads(128)) void paged_append_hd128(PagedRowsArgs a) { append_block<128>(a); }
 
 // Reads one block's rows of a range back as f32; a thread has the codes of the append.
-// Bound by memory: 4 x 2048 rows of 8 heads x 128 in 18.2 us, 84 MB at 4.6 TB/s.
+// Bound by memory: 4 x 2048 rows of 8 heads x 128 in 18.3 us (median of 125 launches; the
+// fastest 16.2), 84 MB at 4.6 to 5.2 TB/s.
 template <int HD>
 __device__ __forceinline__ void read_block(const PagedRowsArgs& a) {
   constexpr int MID = HD / 2, BYTES = kBlk * HD, LANES = MID / 4;
@@ -295,7 +297,8 @@ extern "C" __global__ __launch_bounds__(block_threads(128)) void paged_read_hd12
 //                  its largest magnitude, in three signed bytes, so the sums are
 //                  exact; a score is off by the rounding of q (2^-23 of its
 //                  largest value), by less than a step of 2^-14 of it and the
-//                  block's, and by two f32 roundings.
+//                  block's (the lowest byte's sum is rounded down, so always to one
+//                  side), and by two f32 roundings.
 //   softmax        online per column, exp2 of log2(e)-scaled scores.
 //   O^T += V^T P^T v_mfma_f32_16x16x32_f16: the V codes as f16 (a byte placed in
 //                  1024 + code + 128, less 1152), p times the block's scale as f16
@@ -619,9 +622,9 @@ __device__ __forceinline__ void join_splits(const PagedAttnArgs& a, const Item& 
 // of them together, 16 lanes a column, while the first tile is on its way.
 // Bound by the stream of codes where they are many: 64 sequences of 1000 to 4000
 // positions, 331 MB, in 57 us (5.8 TB/s; a stream that only reads reaches 7.1); 8 heads
-// of one sequence behind 32 k positions, 67 MB, in 18.1 us, of which the join of 32
+// of one sequence behind 32 k positions, 67 MB, in 18.4 us, of which the join of 32
 // splits is about 4 (one CU reads their results at some 45 GB/s) and start and end 4.
-// Short contexts are a chain of dependent accesses: 7.5 us for 512 positions.  32 and 48
+// Short contexts are a chain of dependent accesses: 7.3 us for 512 positions.  32 and 48
 // columns per workgroup read the cache less often and were slower at every size tried (16
 // sequences, 5 rows of 4 heads behind 2100 positions: 22.8 us with 16, 27.5 and 48.4), as
 // were three waves per SIMD (57 us became 60; registers spill).
@@ -793,7 +796,7 @@ __device__ __forceinline__ void attend_few(const PagedAttnArgs& a) {
 // Bound by issue: a tile of 16 columns is 56 matrix instructions, 17 exp2 and about 220
 // others, which in a loop of two or three waves per SIMD cost 8, 9.6 and 4.4 cycles of
 // it: 1590 of the 2175 that a tile takes.  2048 rows of 32 heads behind 2048 positions
-// are 183 to 200 us, 103 GFLOP of the formula.  No faster were 128 columns in eight waves,
+// are 187 to 199 us (the fastest and the median of 125 launches), 103 GFLOP of the formula.  No faster were 128 columns in eight waves,
 // 32 columns per wave (346 us: registers spill; 64 dims: 150 against 136), the next tile's
 // scores among this one's weights (205 to 215) and raised priority of the matrix
 // instructions (208).

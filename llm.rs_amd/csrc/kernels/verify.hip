@@ -6,9 +6,11 @@
 // p(x) and draft probability q(x), is accepted while u_j q(x) < p(x): the product
 // of two f32 values is exact in 64 bits, so no rounding decides.  The first
 // refusal draws from max(p - q, 0), a sequence without one from the target row
-// after its last draft: the smallest id whose running sum (64 bits, index order)
-// exceeds draw * total.  Where nothing is left of the target, it is drawn from as
-// it is.
+// after its last draft: the smallest id whose running sum exceeds draw * total.
+// The sums are 64 bits and of one order (eight ids of a lane in turn, the lanes and
+// then the slices as trees), so the id is that of the formula where the draw does not
+// meet a running sum to within their roundings, and always one that has something.
+// Where nothing is left of the target, it is drawn from as it is.
 #include "common.h"
 #include "../kernel_args.h"
 
@@ -224,9 +226,10 @@ __device__ __forceinline__ int draw(const VerifyArgs& a, const Row& r, const uns
 // waiting; the sums move with device-scope stores and loads) draws, one wave of it
 // alone: the slice in which the running sum crosses, and the id in that slice.  Its
 // answer goes straight to the host's memory, where the caller waits for the stamps.
-// Bound by latency (words, drafted ids, row, sums, ticket, sums, slice): 5.7 us for one
-// sequence of 32000 ids, 8.3 us for 32 of 128256 with drafts' probabilities (33 MB);
-// tickets next to each other in memory made that 34.
+// Bound by latency (words, drafted ids, row, sums, ticket, sums, slice): 5.9 us (median
+// of 125 launches; the fastest 5.5) for one sequence of 32000 ids, 8.3 us (7.7) for 32 of
+// 128256 with drafts' probabilities (33 MB); tickets next to each other in memory made
+// that 34.
 extern "C" __global__ __launch_bounds__(kThreads) void verify_rows(VerifyArgs a) {
   const int i = blockIdx.y, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(wave_id());
   const Row r = examine(a, i);

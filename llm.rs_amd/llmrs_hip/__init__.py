@@ -847,7 +847,9 @@ class HipPagedCache:
         return int(n.value)
 
     def truncate(self, slots, lengths) -> None:
-        """Shortens sequences to the given lengths."""
+        """Shortens sequences to the given lengths.  The rows that stay keep the
+        codes and scales they have: a row that is taken back may have left
+        those of its block coarser."""
         slots, lengths = _pair(slots, lengths, "truncate")
         _check(lib().llmrs_paged_truncate(self._h, _ref(slots), _ref(lengths), slots.size))
 
